@@ -5,9 +5,17 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "mmn_kernels.hip")
+CSRC = os.path.join(HERE, "csrc")
+SRC = os.path.join(CSRC, "mmn_kernels.hip")
 INC = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "libmmn_hip.so")
+OBJ = os.path.join(os.path.dirname(HERE), "build")
+HEADERS = ("mmn_hip.h", "mmn_sequence.h")
+#: the library's translation units, compiled side by side
+UNITS = ("mmn_kernels.hip", "mmn_sequence.hip", "mmn_scan.hip")
+#: packed 32-bit float operations off: some of their forms have given wrong results on this hardware
+_NO_PACKED = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
+UNIT_FLAGS = {unit: _NO_PACKED for unit in ("mmn_sequence.hip", "mmn_scan.hip")}
 
 
 def hipcc_path() -> str:
@@ -18,8 +26,7 @@ def hipcc_path() -> str:
 
 
 def source_files():
-    csrc = os.path.dirname(SRC)                           # mmn_kernels.hip includes the *.inc files next to it
-    return sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".hip", ".inc"))) + [os.path.join(INC, "mmn_hip.h")]
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".inc"))) + [os.path.join(INC, h) for h in HEADERS]
 
 
 def source_hash() -> str:
@@ -58,19 +65,34 @@ def needs_build() -> bool:
     return not os.path.exists(OUT) or built_hash() != source_hash()
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
+def build(force: bool = False, verbose: bool = False, only=None) -> str:
+    """Compile and link.  `only`: compile these units and take the others' objects as they are (a developer's shortcut)."""
     if not force and not needs_build():
         return OUT
     # -amdgpu-mfma-vgpr-form: accumulators stay in VGPRs (gfx950's register file is unified).  With AGPR accumulators
     # hipcc rotated k_wgrad's sixteen accumulator tiles through v_accvgpr_read / _write pairs in every unrolled loop
     # body (reads that wait for the MFMA that produced the tile): k_wgrad 18.1 -> 17.5 us, the step -1.4 us.
-    cmd = [hipcc_path(), "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-shared", "-mllvm", "-amdgpu-mfma-vgpr-form",
-           f'-DMMN_SOURCE_HASH="{source_hash()}"', f"-I{INC}", SRC, "-o", OUT]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    flags = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-mfma-vgpr-form", f"-I{INC}"]
+    os.makedirs(OBJ, exist_ok=True)
+    objects, running = [], []
+    for unit in UNITS:
+        obj = os.path.join(OBJ, unit.replace(".hip", ".o"))
+        cmd = [hipcc_path(), *flags, *UNIT_FLAGS.get(unit, ()), "-c", os.path.join(CSRC, unit), "-o", obj]
+        if unit == "mmn_sequence.hip":                     # (the unit that says what the library was built from: a quick one)
+            cmd.insert(1, f'-DMMN_SOURCE_HASH="{source_hash()}"')
+        objects.append(obj)
+        if only is not None and unit not in only and os.path.exists(obj):
+            continue
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        running.append((unit, subprocess.Popen(cmd)))
+    failed = [unit for unit, p in running if p.wait() != 0]
+    if failed:
+        raise RuntimeError(f"hipcc failed on {', '.join(failed)}")
+    subprocess.run([hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", OUT], check=True)
     return OUT
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
+    units = [a for a in sys.argv[1:] if a in UNITS]
+    print(build(force="--force" in sys.argv or bool(units), verbose=True, only=units or None))

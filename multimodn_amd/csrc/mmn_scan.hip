@@ -1,0 +1,179 @@
+// mmn_scan.hip -- gfx950 kernels and C entry points of the selective scan (include/mmn_sequence.h).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <stdlib.h>
+
+#include "mmn_hip.h"
+#include "mmn_sequence.h"
+
+namespace {
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+#include "seq_common.inc"
+#include "seq_sum.inc"
+#include "seq_scan.inc"
+}  // namespace
+
+#include "seq_host.inc"
+
+static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
+static int mark_every(int n) { return padded_states(n) >= 32 ? ScanShape<32>::CK : ScanShape<16>::CK; }
+
+struct ScanPlan {
+    int waves, cblocks, seg, nseg, nmark;
+    int64_t grid;
+    size_t off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
+};
+static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
+    ScanPlan p;
+    const int per = s->width / s->groups, tiles = (int)ceil_div(per, 64);
+    // Waves a workgroup: as few lanes without a channel as there can be, then as few workgroups
+    int best = 1 << 30;
+    p.waves = 1;
+    for (int w = 1; w <= 4; ++w) {
+        const int blocks = (int)ceil_div(tiles, w), cost = 4 * blocks * w + blocks;
+        if (cost < best) { best = cost; p.waves = w; }
+    }
+    p.cblocks = (int)ceil_div(tiles, p.waves);
+    // Segments: until there are two waves for each of the 1024 SIMDs
+    const int64_t waves = s->batch * s->groups * tiles, want = ceil_div(2048, waves > 0 ? waves : 1);
+    const int64_t most = ceil_div(s->steps, SCAN_SEG), n = want < most ? want : most;
+    p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), SCAN_SEG) * SCAN_SEG) : (s->steps > 0 ? s->steps : 1);
+    p.nseg = s->steps > 0 ? (int)ceil_div(s->steps, p.seg) : 1;
+    p.nmark = (int)ceil_div(s->steps, mark_every(s->states));
+    p.grid = s->batch * p.nseg * s->groups * p.cblocks;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += pad256(n); return o; };
+    const size_t rows = (size_t)s->batch * p.nseg;
+    p.off_segh = take(p.nseg > 1 ? sizeof(float) * rows * s->states * s->width : 0);
+    p.off_segdt = take(p.nseg > 1 ? sizeof(float) * rows * s->width : 0);
+    p.off_part = p.off_mid = p.off_bc = at;
+    if (backward) {
+        const int64_t n = (int64_t)(s->states + 2) * s->width;
+        p.off_part = take(sizeof(float) * rows * n);
+        p.off_mid = take(sum_parts_bytes((int64_t)rows, n));
+        p.off_bc = take(p.cblocks > 1 ? sizeof(float) * (size_t)p.cblocks * s->batch * s->steps * s->groups * 2 * s->states : 0);
+    }
+    p.bytes = at > 0 ? at : 256;
+    return p;
+}
+
+static bool scan_sizes_ok(const mmn_seq_scan_desc* s) {
+    return s && s->batch >= 0 && s->batch <= MAX_GRID && s->steps >= 0 && s->steps <= (1 << 30) && s->width >= 1 && s->groups >= 1 && s->width % s->groups == 0 &&
+           s->states >= 1 && s->states <= MMN_SEQ_MAX_STATES && s->type >= 0 && s->type <= 2;
+}
+
+static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* ws) {
+    ScanArgs a;
+    a.x = s->x; a.dt = s->dt; a.b = s->b; a.c = s->c; a.z = s->z; a.dy = s->dy;
+    a.a = s->a; a.d = s->d; a.dt_bias = s->dt_bias; a.state = s->state; a.dstate_out = s->dstate_out; a.lengths = s->lengths;
+    a.y = s->y; a.dx = s->dx; a.ddt = s->ddt; a.dz = s->dz; a.db = s->db; a.dc = s->dc;
+    a.state_out = s->state_out; a.dstate = s->dstate;
+    a.seg_h = (float*)(ws + p.off_segh); a.seg_dt = (float*)(ws + p.off_segdt); a.marks = s->marks;
+    a.part = (float*)(ws + p.off_part); a.bc_part = (float*)(ws + p.off_bc);
+    a.batch = s->batch;
+    a.xb = s->x_row; a.xt = s->x_step; a.dtb = s->dt_row; a.dtt = s->dt_step; a.bb = s->b_row; a.bt = s->b_step; a.bg = s->b_group;
+    a.cb = s->c_row; a.ct = s->c_step; a.cg = s->c_group; a.zb = s->z_row; a.zt = s->z_step; a.dyb = s->dy_row; a.dyt = s->dy_step;
+    a.steps = s->steps; a.width = s->width; a.groups = s->groups; a.states = s->states; a.softplus = s->softplus;
+    a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.cblocks = p.cblocks;
+    return a;
+}
+
+template <typename T, int NP>
+static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.grid), block(64 * p.waves);
+    if (p.nseg > 1) {
+        SEQ_LAUNCH((k_scan_part<T, NP, false>), grid, block, 0, st, a);
+        SEQ_LAUNCH((k_scan_link<false>), dim3((unsigned)ceil_div(a.batch * a.states * a.width, 256)), dim3(256), 0, st, a);
+    }
+    if (a.marks) SEQ_LAUNCH((k_scan<T, NP, true>), grid, block, 0, st, a);
+    else SEQ_LAUNCH((k_scan<T, NP, false>), grid, block, 0, st, a);
+    return MMN_OK;
+}
+
+template <typename T, int NP>
+static int scan_backward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.grid), block(64 * p.waves);
+    if (p.nseg > 1) {
+        SEQ_LAUNCH((k_scan_part<T, NP, true>), grid, block, 0, st, a);
+        SEQ_LAUNCH((k_scan_link<true>), dim3((unsigned)ceil_div(a.batch * a.states * a.width, 256)), dim3(256), 0, st, a);
+    }
+    const size_t lds = ScanShape<NP>::grad_lds(p.waves);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_scan_grad<T, NP>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)ScanShape<NP>::grad_lds(4));
+    if (e != hipSuccess) { mmn_note_hip_error((int)e); return MMN_ERR_HIP; }
+    SEQ_LAUNCH((k_scan_grad<T, NP>), grid, block, lds, st, a);
+    if (p.cblocks > 1) {
+        const int64_t rows = a.batch * a.steps * a.groups;
+        SEQ_LAUNCH(k_scan_bc<T>, dim3((unsigned)ceil_div(rows * 2 * a.states, 256)), dim3(256), 0, st, a.bc_part, (T*)a.db, (T*)a.dc, rows, a.states, p.cblocks);
+    }
+    return MMN_OK;
+}
+
+#define SCAN_STATES(FN, T)                                                                                      \
+    (padded_states(s->states) == 4 ? FN<T, 4>(a, p, st) : padded_states(s->states) == 8 ? FN<T, 8>(a, p, st)    \
+     : padded_states(s->states) == 16 ? FN<T, 16>(a, p, st) : FN<T, 32>(a, p, st))
+#define SCAN_TYPES(FN) (s->type == MMN_SEQ_F32 ? SCAN_STATES(FN, float) : s->type == MMN_SEQ_BF16 ? SCAN_STATES(FN, bf16) : SCAN_STATES(FN, f16))
+
+extern "C" {
+
+size_t mmn_seq_scan_marks(const mmn_seq_scan_desc* s) {
+    return scan_sizes_ok(s) ? (size_t)s->batch * scan_plan(s, false).nmark * s->states * s->width : 0;
+}
+
+size_t mmn_seq_scan_bytes(const mmn_seq_scan_desc* s, int backward) { return scan_sizes_ok(s) ? scan_plan(s, backward != 0).bytes : 0; }
+
+int mmn_seq_scan(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* stream) {
+    if (!scan_sizes_ok(s)) return MMN_ERR_ARG;
+    if (s->batch == 0) return MMN_OK;
+    if (!s->a || (s->steps > 0 && (!s->x || !s->dt || !s->b || !s->c || !s->y))) return MMN_ERR_ARG;
+    const ScanPlan p = scan_plan(s, false);
+    if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
+    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 256) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    const hipStream_t st = (hipStream_t)stream;
+    const ScanArgs a = scan_args(s, p, (char*)ws);
+    return SCAN_TYPES(scan_forward);
+}
+
+int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* stream) {
+    if (!scan_sizes_ok(s)) return MMN_ERR_ARG;
+    if (s->batch == 0 || s->steps == 0) return MMN_ERR_UNSUPPORTED;
+    if (!s->a || !s->x || !s->dt || !s->b || !s->c || !s->marks || !s->dy || !s->dx || !s->ddt || !s->db || !s->dc || !s->dparams ||
+        (s->z && !s->dz)) return MMN_ERR_ARG;
+    const ScanPlan p = scan_plan(s, true);
+    if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
+    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 256) > MAX_GRID ||
+        ceil_div(s->batch * s->steps * s->groups * 2 * s->states, 256) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    const hipStream_t st = (hipStream_t)stream;
+    const ScanArgs a = scan_args(s, p, (char*)ws);
+    const int rc = SCAN_TYPES(scan_backward);
+    if (rc != MMN_OK) return rc;
+    return sum_parts(a.part, (float*)((char*)ws + p.off_mid), s->dparams, s->batch * p.nseg, (int64_t)(s->states + 2) * s->width, s->width, s->states, st);
+}
+
+int mmn_seq_scan_step(const mmn_seq_scan_desc* s, void* stream) {
+    if (!scan_sizes_ok(s)) return MMN_ERR_ARG;
+    if (s->batch == 0) return MMN_OK;
+    if (!s->a || !s->x || !s->dt || !s->b || !s->c || !s->y || !s->state || !s->state_out) return MMN_ERR_ARG;
+    const hipStream_t st = (hipStream_t)stream;
+    ScanPlan p = {};
+    ScanArgs a = scan_args(s, p, nullptr);
+    // four states a lane where every channel's begin on 16 bytes
+    const bool four = s->states % 4 == 0 && aligned(s->state, 16) && aligned(s->state_out, 16) && aligned(s->a, 16);
+    const int q = log2_up(ceil_div(s->states, four ? 4 : 1), 5);
+    const int64_t gx = ceil_div((s->batch * s->width) << q, 256);
+    if (gx > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)gx);
+#define STEP(T)                                                                                  \
+    do {                                                                                         \
+        if (four) SEQ_LAUNCH((k_scan_step<T, 4>), grid, dim3(256), 0, st, a, q);                 \
+        else SEQ_LAUNCH((k_scan_step<T, 1>), grid, dim3(256), 0, st, a, q);                      \
+    } while (0)
+    if (s->type == MMN_SEQ_F32) STEP(float);
+    else if (s->type == MMN_SEQ_BF16) STEP(bf16);
+    else STEP(f16);
+#undef STEP
+    return MMN_OK;
+}
+
+}  // extern "C"

@@ -42,6 +42,12 @@ ABI_SYMBOLS = (
     "mmn_epoch_small_rows", "mmn_train_epoch_small", "mmn_dp_oneshot_detach", "mmn_per_sample_supported", "mmn_dp_oneshot_diag",
 )
 
+#: every symbol include/mmn_sequence.h declares
+SEQUENCE_SYMBOLS = (
+    "mmn_seq_embed", "mmn_seq_embed_grad_bytes", "mmn_seq_embed_grad", "mmn_seq_conv", "mmn_seq_conv_grad_bytes", "mmn_seq_conv_grad",
+    "mmn_seq_conv_step", "mmn_seq_scan_marks", "mmn_seq_scan_bytes", "mmn_seq_scan", "mmn_seq_scan_grad", "mmn_seq_scan_step",
+)
+
 
 class Linear(C.Structure):
     _fields_ = [("w", C.c_void_p), ("b", C.c_void_p), ("gw", C.c_void_p), ("gb", C.c_void_p),
@@ -82,6 +88,21 @@ class AdamDesc(C.Structure):
                 ("weight_decay", C.c_double), ("n_seg", C.c_int32), ("maximize", C.c_int32)]
 
 
+class ConvDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "state", "y", "state_out", "weight", "bias", "lengths", "dy", "dstate_out", "dx", "dstate",
+                                          "dweight", "dbias")] + \
+               [(n, C.c_int64) for n in ("batch", "x_row", "x_step", "dy_row", "dy_step")] + \
+               [(n, C.c_int32) for n in ("steps", "width", "taps", "silu", "type", "reserved")]
+
+
+class ScanDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "dt", "b", "c", "z", "a", "d", "dt_bias", "state", "lengths", "y", "state_out", "marks", "dy",
+                                          "dstate_out", "dx", "ddt", "db", "dc", "dz", "dparams", "dstate")] + \
+               [(n, C.c_int64) for n in ("batch", "x_row", "x_step", "dt_row", "dt_step", "b_row", "b_step", "b_group", "c_row", "c_step",
+                                         "c_group", "z_row", "z_step", "dy_row", "dy_step")] + \
+               [(n, C.c_int32) for n in ("steps", "width", "groups", "states", "softplus", "type")]
+
+
 class StepOpts(C.Structure):
     _fields_ = [("adam", C.POINTER(AdamDesc)), ("next", C.POINTER(Batch)), ("accumulate_epoch", C.c_int32),
                 ("reserved", C.c_int32), ("next_drop_p", C.POINTER(C.c_float)), ("next_drop_buf", C.c_void_p),
@@ -112,7 +133,7 @@ def load(path: Optional[str] = None) -> C.CDLL:
             f"__graft_entry__ as g; g.build()'` (needs hipcc). There is no CPU fallback for the "
             f"training hot path.")
     lib = C.CDLL(p)
-    missing = [s for s in ABI_SYMBOLS if not hasattr(lib, s)]
+    missing = [s for s in ABI_SYMBOLS + SEQUENCE_SYMBOLS if not hasattr(lib, s)]
     if missing:
         raise MmnError(f"{p} does not export {missing}")
     vp, i32, f32 = C.c_void_p, C.c_int, C.c_float
@@ -228,6 +249,14 @@ def load(path: Optional[str] = None) -> C.CDLL:
     lib.mmn_dropout_adopt.argtypes = [vp, C.POINTER(Batch), C.POINTER(C.c_float), vp, C.c_size_t, vp]
     lib.mmn_dropout_reset.restype = i32
     lib.mmn_dropout_reset.argtypes = [vp, vp]
+    i64, size, conv, scan = C.c_int64, C.c_size_t, C.POINTER(ConvDesc), C.POINTER(ScanDesc)
+    for name, res, args in (
+            ("mmn_seq_embed", i32, [vp, i32, vp, vp, i64, i64, i32, i32, f32, vp]), ("mmn_seq_embed_grad_bytes", size, [i64, i64, i32]),
+            ("mmn_seq_embed_grad", i32, [vp, i32, vp, vp, i64, i64, i32, i32, f32, vp, size, vp]),
+            ("mmn_seq_conv", i32, [conv, vp]), ("mmn_seq_conv_grad_bytes", size, [conv]), ("mmn_seq_conv_grad", i32, [conv, vp, size, vp]),
+            ("mmn_seq_conv_step", i32, [conv, vp]), ("mmn_seq_scan_marks", size, [scan]), ("mmn_seq_scan_bytes", size, [scan, i32]),
+            ("mmn_seq_scan", i32, [scan, vp, size, vp]), ("mmn_seq_scan_grad", i32, [scan, vp, size, vp]), ("mmn_seq_scan_step", i32, [scan, vp])):
+        getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
     if lib.mmn_version() != VERSION:
         raise MmnError(f"{p}: ABI version {lib.mmn_version()} != expected {VERSION}; rebuild")
     lib.mmn_source_hash.restype = C.c_char_p
