@@ -81,7 +81,7 @@ def build(force: bool = False, verbose: bool = False, only=None) -> str:
         if unit == "mmn_sequence.hip":                     # (the unit that says what the library was built from: a quick one)
             cmd.insert(1, f'-DMMN_SOURCE_HASH="{source_hash()}"')
         objects.append(obj)
-        if only is not None and unit not in only and os.path.exists(obj):
+        if only is not None and unit not in only and unit != "mmn_sequence.hip" and os.path.exists(obj):
             continue
         if verbose:
             print(" ".join(cmd), flush=True)

@@ -3,6 +3,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <stdlib.h>
+#include <initializer_list>
 
 #include "mmn_hip.h"
 #include "mmn_sequence.h"
@@ -17,12 +18,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 #include "seq_host.inc"
 
 static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
-static int mark_every(int n) { return padded_states(n) >= 32 ? ScanShape<32>::CK : ScanShape<16>::CK; }
 
 struct ScanPlan {
     int waves, cblocks, seg, nseg, nmark;
     int64_t grid;
-    size_t off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
+    bool order;
+    size_t off_order, off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
 };
 static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     ScanPlan p;
@@ -35,16 +36,29 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
         if (cost < best) { best = cost; p.waves = w; }
     }
     p.cblocks = (int)ceil_div(tiles, p.waves);
-    // Segments: until there are two waves for each of the 1024 SIMDs
-    const int64_t waves = s->batch * s->groups * tiles, want = ceil_div(2048, waves > 0 ? waves : 1);
-    const int64_t most = ceil_div(s->steps, SCAN_SEG), n = want < most ? want : most;
+    // Segments, each of which costs a first pass over its steps: enough for two waves on each of the 1024 SIMDs (all that fit of the
+    // backward kernel), half as many again where rows differ in length (4 rows of up to 2048 steps, 1024 channels: 241 us forward and
+    // backward with 3072 waves, 270 with 2048, 248 with 4096).  From 896 waves on the rows are enough by themselves (512 steps, 64
+    // channels, fp32: 600 rows 790 us in segments and 965 in one piece; 1000 rows 1071 and 1045; 1500 rows 1631 and 1511).
+    const int64_t waves = s->batch * s->groups * tiles;
+    const int64_t want = waves >= 896 ? 1 : ceil_div(s->lengths ? 3072 : 2048, waves > 0 ? waves : 1);
+    int64_t n = ceil_div(s->steps, SCAN_SEG);
+    n = want < n ? want : n;
+    // ... and as many as it takes for a segment of the widest strided tensor to stay below 2^30 bytes (32-bit offsets in the kernels)
+    int64_t stride = s->width;
+    for (const int64_t t : {s->x_step, s->dt_step, s->z ? s->z_step : 0, backward ? s->dy_step : 0}) stride = t > stride ? t : stride;
+    const int64_t fits = ((int64_t)1 << 30) / (stride * 4) / SCAN_SEG * SCAN_SEG;
+    if (fits > 0 && ceil_div(s->steps, fits) > n) n = ceil_div(s->steps, fits);
     p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), SCAN_SEG) * SCAN_SEG) : (s->steps > 0 ? s->steps : 1);
     p.nseg = s->steps > 0 ? (int)ceil_div(s->steps, p.seg) : 1;
-    p.nmark = (int)ceil_div(s->steps, mark_every(s->states));
+    p.nmark = (int)ceil_div(s->steps, SCAN_CK);
     p.grid = s->batch * p.nseg * s->groups * p.cblocks;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += pad256(n); return o; };
     const size_t rows = (size_t)s->batch * p.nseg;
+    // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and twice 5.4 for the order, instead of 58 + 175)
+    p.order = s->lengths && p.nseg == 1 && waves >= 896;
+    p.off_order = take(p.order ? sizeof(int32_t) * (size_t)s->batch : 0);
     p.off_segh = take(p.nseg > 1 ? sizeof(float) * rows * s->states * s->width : 0);
     p.off_segdt = take(p.nseg > 1 ? sizeof(float) * rows * s->width : 0);
     p.off_part = p.off_mid = p.off_bc = at;
@@ -62,6 +76,12 @@ static bool scan_sizes_ok(const mmn_seq_scan_desc* s) {
     return s && s->batch >= 0 && s->batch <= MAX_GRID && s->steps >= 0 && s->steps <= (1 << 30) && s->width >= 1 && s->groups >= 1 && s->width % s->groups == 0 &&
            s->states >= 1 && s->states <= MMN_SEQ_MAX_STATES && s->type >= 0 && s->type <= 2;
 }
+// A segment of at least SCAN_SEG steps is addressed with 32-bit offsets; steps that share memory would not read as 0 behind the end
+static bool scan_strides_ok(const mmn_seq_scan_desc* s, bool backward) {
+    const int64_t most = 1 << 23;
+    auto ok = [&](int64_t stride) { return (stride >= s->width || s->steps == 1) && stride >= 0 && stride <= most; };
+    return s->width <= most && ok(s->x_step) && ok(s->dt_step) && (!s->z || ok(s->z_step)) && (!backward || ok(s->dy_step));
+}
 
 static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* ws) {
     ScanArgs a;
@@ -69,6 +89,7 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
     a.a = s->a; a.d = s->d; a.dt_bias = s->dt_bias; a.state = s->state; a.dstate_out = s->dstate_out; a.lengths = s->lengths;
     a.y = s->y; a.dx = s->dx; a.ddt = s->ddt; a.dz = s->dz; a.db = s->db; a.dc = s->dc;
     a.state_out = s->state_out; a.dstate = s->dstate;
+    a.order = p.order ? (const int32_t*)(ws + p.off_order) : nullptr;
     a.seg_h = (float*)(ws + p.off_segh); a.seg_dt = (float*)(ws + p.off_segdt); a.marks = s->marks;
     a.part = (float*)(ws + p.off_part); a.bc_part = (float*)(ws + p.off_bc);
     a.batch = s->batch;
@@ -82,9 +103,12 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
 template <typename T, int NP>
 static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid), block(64 * p.waves);
+    if (p.order) SEQ_LAUNCH(k_scan_order, dim3(1), dim3(1024), 0, st, a.lengths, const_cast<int32_t*>(a.order), (int)a.batch, a.steps);
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, false>), grid, block, 0, st, a);
-        SEQ_LAUNCH((k_scan_link<false>), dim3((unsigned)ceil_div(a.batch * a.states * a.width, 256)), dim3(256), 0, st, a);
+        const int64_t lanes = a.batch * a.states * a.width;
+        if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<false, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
+        else SEQ_LAUNCH((k_scan_link<false, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
     if (a.marks) SEQ_LAUNCH((k_scan<T, NP, true>), grid, block, 0, st, a);
     else SEQ_LAUNCH((k_scan<T, NP, false>), grid, block, 0, st, a);
@@ -94,9 +118,12 @@ static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
 template <typename T, int NP>
 static int scan_backward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid), block(64 * p.waves);
+    if (p.order) SEQ_LAUNCH(k_scan_order, dim3(1), dim3(1024), 0, st, a.lengths, const_cast<int32_t*>(a.order), (int)a.batch, a.steps);
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, true>), grid, block, 0, st, a);
-        SEQ_LAUNCH((k_scan_link<true>), dim3((unsigned)ceil_div(a.batch * a.states * a.width, 256)), dim3(256), 0, st, a);
+        const int64_t lanes = a.batch * a.states * a.width;
+        if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<true, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
+        else SEQ_LAUNCH((k_scan_link<true, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
     const size_t lds = ScanShape<NP>::grad_lds(p.waves);
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_scan_grad<T, NP>), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -127,9 +154,10 @@ int mmn_seq_scan(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* st
     if (!scan_sizes_ok(s)) return MMN_ERR_ARG;
     if (s->batch == 0) return MMN_OK;
     if (!s->a || (s->steps > 0 && (!s->x || !s->dt || !s->b || !s->c || !s->y))) return MMN_ERR_ARG;
+    if (!scan_strides_ok(s, false)) return MMN_ERR_UNSUPPORTED;
     const ScanPlan p = scan_plan(s, false);
     if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
-    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 256) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 64) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
     const ScanArgs a = scan_args(s, p, (char*)ws);
     return SCAN_TYPES(scan_forward);
@@ -140,9 +168,10 @@ int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, voi
     if (s->batch == 0 || s->steps == 0) return MMN_ERR_UNSUPPORTED;
     if (!s->a || !s->x || !s->dt || !s->b || !s->c || !s->marks || !s->dy || !s->dx || !s->ddt || !s->db || !s->dc || !s->dparams ||
         (s->z && !s->dz)) return MMN_ERR_ARG;
+    if (!scan_strides_ok(s, true)) return MMN_ERR_UNSUPPORTED;
     const ScanPlan p = scan_plan(s, true);
     if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
-    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 256) > MAX_GRID ||
+    if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 64) > MAX_GRID ||
         ceil_div(s->batch * s->steps * s->groups * 2 * s->states, 256) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
     const ScanArgs a = scan_args(s, p, (char*)ws);

@@ -50,7 +50,7 @@ int mmn_seq_embed(const void* ids, int ids64, const void* table, void* out, int6
 
 struct EmbedGradPlan {
     int passes, bits, bins, nwg, run, chunk, nchunk, v, ctiles;
-    size_t off_hist, off_clear, nclear, off_present, off_keys[2], off_pos[2], off_part, bytes;
+    size_t off_hist, off_present, off_keys[2], off_pos[2], off_part, bytes;
 };
 // `v`: elements a lane sums (the partial sums' size does not depend on it)
 static EmbedGradPlan embed_grad_plan(int64_t rows, int64_t vocab, int width) {
@@ -73,11 +73,7 @@ static EmbedGradPlan embed_grad_plan(int64_t rows, int64_t vocab, int width) {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += pad256(n); return o; };
     p.off_hist = take(sizeof(unsigned) * (size_t)p.nwg * p.bins);
-    const size_t next = (size_t)(p.passes - 1) * p.nwg * p.bins;
-    p.off_clear = at;                                    // cleared together: the later passes' counts, then the marks of present ids
-    p.nclear = next + (size_t)vocab;
-    take(sizeof(unsigned) * p.nclear);
-    p.off_present = p.off_clear + sizeof(unsigned) * next;
+    p.off_present = take(sizeof(unsigned) * (size_t)vocab);
     for (int i = 0; i < 2; ++i) {
         p.off_keys[i] = take(sizeof(unsigned) * (size_t)rows);
         p.off_pos[i] = take(sizeof(unsigned) * (size_t)rows);
@@ -102,25 +98,23 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
     const hipStream_t st = (hipStream_t)stream;
     char* w = (char*)ws;
     unsigned* hist = (unsigned*)(w + p.off_hist);
-    unsigned* clear = (unsigned*)(w + p.off_clear);
     unsigned* present = (unsigned*)(w + p.off_present);
     unsigned *keys[2], *pos[2];
     for (int i = 0; i < 2; ++i) { keys[i] = (unsigned*)(w + p.off_keys[i]); pos[i] = (unsigned*)(w + p.off_pos[i]); }
     float* part = (float*)(w + p.off_part);
     const int nwg = rows > 0 ? p.nwg : 0;
-    const int clear_wg = (int)ceil_div((int64_t)p.nclear, SORT_NT * 8) < 256 ? (int)ceil_div((int64_t)p.nclear, SORT_NT * 8) : 256;
-    const dim3 hg(nwg + clear_wg), nt(SORT_NT);
-    if (ids64) SEQ_LAUNCH(k_sort_hist<int64_t>, hg, nt, 0, st, (const int64_t*)ids, rows, (int)vocab, p.run, nwg, p.bins, hist, clear, (int64_t)p.nclear);
-    else SEQ_LAUNCH(k_sort_hist<int32_t>, hg, nt, 0, st, (const int32_t*)ids, rows, (int)vocab, p.run, nwg, p.bins, hist, clear, (int64_t)p.nclear);
+    const int64_t clear_wg = ceil_div(vocab, SORT_NT * 8) < 256 ? ceil_div(vocab, SORT_NT * 8) : 256;
+    const dim3 hg((unsigned)(nwg + clear_wg)), nt(SORT_NT);
+    if (ids64) SEQ_LAUNCH((k_sort_hist<int64_t, true>), hg, nt, 0, st, (const int64_t*)ids, nullptr, rows, (int)vocab, p.run, nwg, p.bins, 0, hist, present, vocab);
+    else SEQ_LAUNCH((k_sort_hist<int32_t, true>), hg, nt, 0, st, (const int32_t*)ids, nullptr, rows, (int)vocab, p.run, nwg, p.bins, 0, hist, present, vocab);
     int at = 0;
     for (int i = 0; i < p.passes && rows > 0; ++i) {
-        const unsigned* h = i == 0 ? hist : clear + (size_t)(i - 1) * p.nwg * p.bins;
-        unsigned* next = i + 1 < p.passes ? clear + (size_t)i * p.nwg * p.bins : nullptr;
         if (i == 0) {
-            if (ids64) SEQ_LAUNCH((k_sort_pass<int64_t, true>), dim3(nwg), nt, 0, st, (const int64_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, h, next, present);
-            else SEQ_LAUNCH((k_sort_pass<int32_t, true>), dim3(nwg), nt, 0, st, (const int32_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, h, next, present);
+            if (ids64) SEQ_LAUNCH((k_sort_pass<int64_t, true>), dim3(nwg), nt, 0, st, (const int64_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, hist, present);
+            else SEQ_LAUNCH((k_sort_pass<int32_t, true>), dim3(nwg), nt, 0, st, (const int32_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, hist, present);
         } else {
-            SEQ_LAUNCH((k_sort_pass<int64_t, false>), dim3(nwg), nt, 0, st, nullptr, keys[at], pos[at], keys[1 - at], pos[1 - at], rows, (int)vocab, p.run, p.nwg, p.bits, i * p.bits, h, next, nullptr);
+            SEQ_LAUNCH((k_sort_hist<int64_t, false>), dim3(nwg), nt, 0, st, nullptr, keys[at], rows, (int)vocab, p.run, nwg, p.bins, i * p.bits, hist, nullptr, (int64_t)0);
+            SEQ_LAUNCH((k_sort_pass<int64_t, false>), dim3(nwg), nt, 0, st, nullptr, keys[at], pos[at], keys[1 - at], pos[1 - at], rows, (int)vocab, p.run, p.nwg, p.bits, i * p.bits, hist, nullptr);
             at = 1 - at;
         }
     }
@@ -129,12 +123,12 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
     const int ctiles = (int)ceil_div(width, 64 * v), nchunk = rows > 0 ? p.nchunk : 0;
     const int64_t sumwg = ceil_div((int64_t)nchunk * ctiles, 4);
     const int64_t zero_wg = ceil_div(vocab, 16) < 2048 ? ceil_div(vocab, 16) : 2048;
-    if (sumwg + zero_wg > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    if (sumwg + zero_wg > MAX_GRID || ceil_div(width, 64) > 65535) return MMN_ERR_UNSUPPORTED;
     const dim3 sg((unsigned)(sumwg + zero_wg));
 #define SUM(T, V)                                                                                                                \
     do {                                                                                                                         \
         SEQ_LAUNCH((k_embed_sum<T, V>), sg, dim3(256), 0, st, keys[at], pos[at], (const T*)grad, (T*)out, part, present, rows, (int)vocab, width, p.chunk, nchunk, ctiles, sumwg, scale); \
-        if (nchunk > 1) SEQ_LAUNCH(k_embed_join<T>, dim3(nchunk - 1), dim3(256), 0, st, keys[at], part, (T*)out, rows, (int)vocab, width, p.chunk, nchunk, scale); \
+        if (nchunk > 1) SEQ_LAUNCH(k_embed_join<T>, dim3((unsigned)ceil_div(nchunk, JOIN_WAVES), (unsigned)ceil_div(width, 64)), dim3(64 * JOIN_WAVES), 0, st, keys[at], part, (T*)out, rows, (int)vocab, width, p.chunk, nchunk, scale); \
     } while (0)
     if (type == MMN_SEQ_F32) { if (v == 4) SUM(float, 4); else SUM(float, 1); }
     else if (type == MMN_SEQ_BF16) { if (v == 8) SUM(bf16, 8); else if (v == 2) SUM(bf16, 2); else SUM(bf16, 1); }

@@ -52,7 +52,14 @@ def _gpu(first: Tensor, **others: Optional[Tensor]) -> int:
 def _data(name: str, t: Tensor, dtype: torch.dtype, *shape: int) -> Tensor:
     _need(isinstance(t, Tensor) and t.dtype == dtype, f"{name} must be a {dtype} tensor, as the other data of the call")
     _need(tuple(t.shape) == shape, f"{name} must be {list(shape)}, not {list(t.shape)}")
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 and t.is_contiguous() else t.contiguous()
+    # (the kernels address a few steps of a row with 32-bit offsets: steps further apart than 2^23 elements are brought together, steps
+    #  that share memory taken apart)
+    if t.stride(-1) == 1:
+        step = t.stride(1) if len(shape) > 2 else shape[-1]
+        if shape[-1] <= step <= 1 << 23 or shape[1] <= 1:
+            return t
+        return t.clone(memory_format=torch.contiguous_format)
+    return t.contiguous()
 
 
 def _float(name: str, t: Optional[Tensor], *shape: int) -> Optional[Tensor]:

@@ -8,8 +8,8 @@ with tempfile.TemporaryDirectory() as td:
     tmp = os.path.join(td, "lib.so")
     subprocess.run(["cp", so, tmp], check=True)
     subprocess.run([f"{llvm}/llvm-objdump", "--offloading", tmp], check=True, capture_output=True)
-    co = [f for f in os.listdir(td) if "gfx950" in f][0]
-    txt = subprocess.run([f"{llvm}/llvm-readelf", "--notes", os.path.join(td, co)], check=True, capture_output=True, text=True).stdout
+    txt = "".join(subprocess.run([f"{llvm}/llvm-readelf", "--notes", os.path.join(td, f)], check=True, capture_output=True, text=True).stdout
+                  for f in sorted(os.listdir(td)) if "gfx950" in f)                     # (one code object for each translation unit)
     dem = {}
     rows = []
     for blk in txt.split("- .agpr_count")[1:]:
