@@ -9,6 +9,7 @@ CSRC = os.path.join(HERE, "csrc")
 SRC = os.path.join(CSRC, "mmn_kernels.hip")
 INC = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "libmmn_hip.so")
+BINDING = os.path.join(HERE, "_binding.so")
 OBJ = os.path.join(os.path.dirname(HERE), "build")
 HEADERS = ("mmn_hip.h", "mmn_sequence.h")
 #: the library's translation units, compiled side by side
@@ -26,7 +27,7 @@ def hipcc_path() -> str:
 
 
 def source_files():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".inc"))) + [os.path.join(INC, h) for h in HEADERS]
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".inc", ".cpp"))) + [os.path.join(INC, h) for h in HEADERS]
 
 
 def source_hash() -> str:
@@ -62,7 +63,22 @@ def built_hash(path: str = OUT):
 
 
 def needs_build() -> bool:
-    return not os.path.exists(OUT) or built_hash() != source_hash()
+    if not os.path.exists(OUT) or not os.path.exists(BINDING) or built_hash() != source_hash():
+        return True
+    with open(BINDING, "rb") as f:                         # (the hash is a string constant of the binding)
+        return source_hash().encode() not in f.read()
+
+
+def binding_command():
+    """g++ on csrc/binding.cpp against this interpreter's torch."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], INC)]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-DTORCH_EXTENSION_NAME=_binding", f'-DMMN_SOURCE_HASH="{source_hash()}"', *inc, os.path.join(CSRC, "binding.cpp"),
+            f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl", f"-Wl,-rpath,{lib}", "-o", BINDING]
 
 
 def build(force: bool = False, verbose: bool = False, only=None) -> str:
@@ -86,9 +102,12 @@ def build(force: bool = False, verbose: bool = False, only=None) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         running.append((unit, subprocess.Popen(cmd)))
+    if verbose:
+        print(" ".join(binding_command()), flush=True)
+    running.append(("binding.cpp", subprocess.Popen(binding_command())))
     failed = [unit for unit, p in running if p.wait() != 0]
     if failed:
-        raise RuntimeError(f"hipcc failed on {', '.join(failed)}")
+        raise RuntimeError(f"the compiler failed on {', '.join(failed)}")
     subprocess.run([hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", *objects, "-o", OUT], check=True)
     return OUT
 

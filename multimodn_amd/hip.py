@@ -277,3 +277,29 @@ def check(rc: int, what: str) -> None:
         msg = lib.mmn_error_string(rc).decode()
         extra = f" (hipError {lib.mmn_last_hip_error()})" if rc == -4 else ""
         raise MmnError(f"{what} failed: {msg}{extra}")
+
+
+_binding = None
+
+
+def load_binding():
+    """The native binding of the sequence operators (csrc/binding.cpp), bound to the loaded library.  Raises if it is absent or was
+    built from other sources."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    load()
+    path = os.environ.get("MMN_LIB_PATH") or LIB_PATH
+    try:
+        from . import _binding as m
+    except ImportError as e:
+        raise MmnError(f"the sequence operators' binding is not built ({e}). Run `python -c 'import __graft_entry__ as g; g.build()'`") from e
+    if not os.environ.get("MMN_LIB_PATH"):
+        from . import build as _build
+        want, have = _build.source_hash(), m.source_hash()
+        if have != want:
+            raise MmnError(f"{m.__file__} was built from other sources (binding {have}, tree {want}): run `python -m multimodn_amd.build`")
+    import torch
+    m.bind(path, MmnError, torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None, check)
+    _binding = m
+    return m

@@ -474,6 +474,10 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert lib.mmn_seq_scan(C.byref(s), 256, 1 << 40, None) == ARG and lib.mmn_seq_scan_step(C.byref(s), None) == ARG
     for name in ("x", "dt", "b", "c", "a", "y"):
         setattr(s, name, 256)
+    assert lib.mmn_seq_scan(C.byref(s), 256, 1 << 40, None) == UNSUPPORTED   # steps that share memory
+    s.x_step = s.dt_step = 1 << 24
+    assert lib.mmn_seq_scan(C.byref(s), 256, 1 << 40, None) == UNSUPPORTED   # steps too far apart
+    s.x_step = s.dt_step = 6
     assert lib.mmn_seq_scan(C.byref(s), None, 0, None) == WORKSPACE
     assert lib.mmn_seq_scan_grad(C.byref(s), 256, 1 << 40, None) == ARG
     s.states = 33
