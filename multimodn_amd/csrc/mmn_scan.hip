@@ -193,10 +193,16 @@ int mmn_seq_scan_step(const mmn_seq_scan_desc* s, void* stream) {
     const int64_t gx = ceil_div((s->batch * s->width) << q, 256);
     if (gx > MAX_GRID) return MMN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)gx);
-#define STEP(T)                                                                                  \
-    do {                                                                                         \
-        if (four) SEQ_LAUNCH((k_scan_step<T, 4>), grid, dim3(256), 0, st, a, q);                 \
-        else SEQ_LAUNCH((k_scan_step<T, 1>), grid, dim3(256), 0, st, a, q);                      \
+    // b and c four at a time too where every row's and group's begin on such a vector
+    const size_t vec = 4 * type_size(s->type);
+    const int bc = four && aligned(s->b, vec) && aligned(s->c, vec) && s->b_row % 4 == 0 && s->c_row % 4 == 0 && s->b_group % 4 == 0 && s->c_group % 4 == 0;
+    // states beyond what the last-level cache (256 MB) holds are not kept there
+    const bool past = (double)s->batch * s->width * s->states * sizeof(float) * (s->state == s->state_out ? 1 : 2) > 200e6;
+#define STEP(T)                                                                                          \
+    do {                                                                                                 \
+        if (four && past) SEQ_LAUNCH((k_scan_step<T, 4, true>), grid, dim3(256), 0, st, a, q, bc);       \
+        else if (four) SEQ_LAUNCH((k_scan_step<T, 4, false>), grid, dim3(256), 0, st, a, q, bc);         \
+        else SEQ_LAUNCH((k_scan_step<T, 1, false>), grid, dim3(256), 0, st, a, q, bc);                   \
     } while (0)
     if (s->type == MMN_SEQ_F32) STEP(float);
     else if (s->type == MMN_SEQ_BF16) STEP(bf16);

@@ -65,9 +65,9 @@ static EmbedGradPlan embed_grad_plan(int64_t rows, int64_t vocab, int width) {
     const int64_t per = ceil_div(tiles, 128);
     p.run = (int)(per * SORT_TILE);
     p.nwg = (int)ceil_div(rows, p.run);
-    // Entries a chunk: 16 where there are few (more waves), up to 512 (fewer partial sums to join)
+    // Entries a chunk: 16 where there are few (more waves), up to 512 (fewer borders to join: 65536 places cost 16 us there with 16)
     int c = 16;
-    while (c < 512 && rows / c > 4096) c *= 2;
+    while (c < 512 && rows / c > 2048) c *= 2;
     p.chunk = c;
     p.nchunk = (int)ceil_div(rows, c);
     size_t at = 0;
@@ -149,14 +149,14 @@ static bool conv_args(const mmn_seq_conv_desc* c, ConvArgs& a) {
            c->batch <= MAX_GRID;
 }
 // elements a thread takes together: all rows of all tensors begin on such a vector
-static int conv_vec(const mmn_seq_conv_desc* c, int most) {
+static int conv_vec(const mmn_seq_conv_desc* c) {
     const int size = type_size(c->type);
     auto fits = [&](int v) {
         const void* ptr[] = {c->x, c->state, c->y, c->state_out, c->dy, c->dstate_out, c->dx, c->dstate};
         for (const void* q : ptr) if (!aligned(q, (size_t)v * size)) return false;
         return c->width % v == 0 && c->x_row % v == 0 && c->x_step % v == 0 && c->dy_row % v == 0 && c->dy_step % v == 0;
     };
-    return most >= 8 && fits(8) ? 8 : fits(4) ? 4 : 1;
+    return fits(4) ? 4 : 1;                              // (8 of 16 bits: 23 us instead of 20 for 8 x 2048 x 1024, fewer waves)
 }
 #define CONV_TAPS(KERN, T, V, ...)                                                   \
     do {                                                                             \
@@ -176,13 +176,14 @@ int mmn_seq_conv(const mmn_seq_conv_desc* c, void* stream) {
     if (!c || !conv_args(c, a)) return MMN_ERR_ARG;
     if (c->batch == 0) return MMN_OK;
     if (!c->weight || (c->steps > 0 && (!c->x || !c->y))) return MMN_ERR_ARG;
-    if (a.tiles == 0) a.tiles = 1;                       // no steps: the state still goes on
+    a.tiles = c->steps > 0 ? (int)ceil_div(c->steps, CONV_AHEAD) : 1;      // (no steps: the state still goes on)
     const hipStream_t st = (hipStream_t)stream;
-    const int v = conv_vec(c, 4);
-    a.lanes_log2 = log2_up(ceil_div(c->width, v), 8);
+    const int v = conv_vec(c);
+    a.lanes_log2 = log2_up(ceil_div(c->width, v), 6);
     const int64_t gx = ceil_div(c->batch * a.tiles, 256 >> a.lanes_log2), gy = ceil_div(ceil_div(c->width, v), 1 << a.lanes_log2);
-    if (gx > MAX_GRID || gy > 65535) return MMN_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (gx * gy > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    a.cblocks = (int)gy;
+    const dim3 grid((unsigned)(gx * gy));
     CONV_TYPES(k_conv, grid, dim3(256), 0, st, a);
     return MMN_OK;
 }
@@ -190,8 +191,8 @@ int mmn_seq_conv(const mmn_seq_conv_desc* c, void* stream) {
 struct ConvGradPlan { int v, lanes_log2, parts, gy; int64_t n; size_t off_mid, bytes; };
 static ConvGradPlan conv_grad_plan(const mmn_seq_conv_desc* c) {
     ConvGradPlan p;
-    p.v = conv_vec(c, 4);
-    p.lanes_log2 = log2_up(ceil_div(c->width, p.v), 8);
+    p.v = conv_vec(c);
+    p.lanes_log2 = log2_up(ceil_div(c->width, p.v), 6);
     p.gy = (int)ceil_div(ceil_div(c->width, p.v), 1 << p.lanes_log2);
     const int64_t jobs = c->batch * ceil_div(c->steps, CONV_RUN), wg = ceil_div(jobs, 256 >> p.lanes_log2);
     const int64_t most = p.gy >= 1024 ? 1 : 1024 / p.gy;  // four workgroups a compute unit; each leaves a partial sum
@@ -225,7 +226,8 @@ int mmn_seq_conv_grad(const mmn_seq_conv_desc* c, void* ws, size_t ws_bytes, voi
     a.lanes_log2 = p.lanes_log2;
     a.parts = p.parts;
     a.part = (float*)ws;
-    const dim3 grid(p.parts, p.gy);
+    a.cblocks = p.gy;
+    const dim3 grid((unsigned)p.parts * p.gy);
     CONV_TYPES(k_conv_grad, grid, dim3(256), 0, st, a);
     return sum_parts(a.part, (float*)((char*)ws + p.off_mid), c->dweight, p.parts, p.n, c->width, c->taps, st);
 }
@@ -236,10 +238,12 @@ int mmn_seq_conv_step(const mmn_seq_conv_desc* c, void* stream) {
     if (c->batch == 0) return MMN_OK;
     if (!c->weight || !c->x || !c->y || !c->state || !c->state_out) return MMN_ERR_ARG;
     const hipStream_t st = (hipStream_t)stream;
-    const int v = conv_vec(c, 4);
-    const int64_t gx = ceil_div(c->batch * (c->width / v), 256);
-    if (gx > MAX_GRID) return MMN_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)gx);
+    const int v = conv_vec(c);
+    a.lanes_log2 = log2_up(ceil_div(c->width, v), 6);
+    const int64_t gx = ceil_div(c->batch, CONV_ROWS * (256 >> a.lanes_log2)), gy = ceil_div(ceil_div(c->width, v), 1 << a.lanes_log2);
+    if (gx * gy > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    a.cblocks = (int)gy;
+    const dim3 grid((unsigned)(gx * gy));
     CONV_TYPES(k_conv_step, grid, dim3(256), 0, st, a);
     return MMN_OK;
 }
