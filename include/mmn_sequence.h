@@ -71,6 +71,10 @@ int mmn_seq_scan(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* st
 int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* stream);
 int mmn_seq_scan_step(const mmn_seq_scan_desc* s, void* stream);
 
+/* dx [rows][width] = dpre [rows][hidden] times weight [hidden][width], all 32-bit and dense, hidden <= 128: the gradient that leaves the
+ * fusion chain at an encoder's input, from its first hidden layer's pre-activation gradients (mmn_debug_buffer kind 7). */
+int mmn_seq_input_grad(const float* dpre, const float* weight, float* dx, int64_t rows, int hidden, int width, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@ namespace {
 #include "seq_embed.inc"
 #include "seq_conv.inc"
 #include "seq_sum.inc"
+#include "seq_input.inc"
 }  // namespace
 
 #include "seq_host.inc"
@@ -245,6 +246,17 @@ int mmn_seq_conv_step(const mmn_seq_conv_desc* c, void* stream) {
     a.cblocks = (int)gy;
     const dim3 grid((unsigned)(gx * gy));
     CONV_TYPES(k_conv_step, grid, dim3(256), 0, st, a);
+    return MMN_OK;
+}
+
+int mmn_seq_input_grad(const float* dpre, const float* weight, float* dx, int64_t rows, int hidden, int width, void* stream) {
+    if (rows < 0 || rows > MAX_GRID || hidden < 1 || hidden > INPUT_HIDDEN || width < 1) return MMN_ERR_ARG;
+    if (rows == 0) return MMN_OK;
+    if (!dpre || !weight || !dx) return MMN_ERR_ARG;
+    const hipStream_t st = (hipStream_t)stream;
+    const int64_t ctiles = ceil_div(width, 64), grid = ceil_div(rows, INPUT_ROWS) * ctiles;
+    if (grid > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    SEQ_LAUNCH(k_input_grad, dim3((unsigned)grid), dim3(256), 0, st, dpre, weight, dx, rows, hidden, width, (int)ctiles);
     return MMN_OK;
 }
 

@@ -4,12 +4,15 @@
 `forward` keeps the module-level contract `encoder(state, x) -> new_state` for users who call a
 plugin directly; `MultiModN.train_epoch` does not call it: it hands the parameters to the HIP
 chain kernels (multimodn_amd/engine.py)."""
+import math
 from abc import ABC, abstractmethod
-from typing import Callable, Optional, Tuple
+from typing import Callable, NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
+
+from . import sequence as seq
 
 
 class MultiModEncoder(nn.Module, ABC):
@@ -108,3 +111,89 @@ class LinearEncoder(SLPEncoder):
 class LogisticEncoder(SLPEncoder):
     def __init__(self, state_size: int, n_features: int):
         super().__init__(state_size, n_features, torch.sigmoid)
+
+
+class SequenceState(NamedTuple):
+    """What SequenceFeatures.step carries from token to token (its tensors move on in place)."""
+    conv: Tensor
+    scan: Tensor
+    total: Tensor
+    count: Tensor
+
+
+class SequenceFeatures(nn.Module):
+    """Token ids [batch, steps] to features [batch, width]: embedding, a projection to the scan's input and gate, a short causal
+    convolution, the selective scan, the mean over the steps.  Each runs in multimodn_amd.sequence's kernels (the projections in
+    torch's), forward and backward; there is no CPU fallback.
+
+    A row ends behind its last id >= 0: pad with -1.  An id outside the vocabulary inside a row is a step without a token (its
+    embedding is 0).  A row without any token has the features 0."""
+
+    def __init__(self, vocabulary: int, width: int, states: int = 16, taps: int = 4, rank: Optional[int] = None,
+                 device: Optional[torch.device] = None):
+        super().__init__()
+        if not 1 <= states <= seq.MAX_STATES or not 2 <= taps <= seq.MAX_TAPS or vocabulary < 1 or width < 1:
+            raise ValueError(f"SequenceFeatures needs 1 to {seq.MAX_STATES} states, 2 to {seq.MAX_TAPS} taps, a vocabulary and a width")
+        self.vocabulary, self.width, self.states, self.taps = vocabulary, width, states, taps
+        self.rank = rank if rank is not None else max(1, width // 16)
+        self.table = nn.Parameter(torch.randn(vocabulary, width, device=device) / math.sqrt(width))
+        self.inputs = nn.Linear(width, 2 * width, bias=False, device=device)
+        self.conv_weight = nn.Parameter((torch.rand(width, taps, device=device) * 2 - 1) / math.sqrt(taps))
+        self.conv_bias = nn.Parameter(torch.zeros(width, device=device))
+        self.select = nn.Linear(width, self.rank + 2 * states, bias=False, device=device)
+        self.spread = nn.Linear(self.rank, width, bias=False, device=device)
+        first = torch.exp(torch.rand(width, device=device) * (math.log(0.1) - math.log(1e-3)) + math.log(1e-3))
+        self.dt_bias = nn.Parameter(first + torch.log(-torch.expm1(-first)))            # softplus(dt_bias) = first
+        self.a_log = nn.Parameter(torch.log(torch.arange(1, states + 1, dtype=torch.float32, device=device)).repeat(width, 1))
+        self.skip = nn.Parameter(torch.ones(width, device=device))
+
+    def _select(self, u: Tensor):
+        dt, b, c = self.select(u).split((self.rank, self.states, self.states), dim=-1)
+        return self.spread(dt), -torch.exp(self.a_log), b, c
+
+    def forward(self, ids: Tensor) -> Tensor:
+        if ids.dim() != 2 or ids.is_floating_point():
+            raise ValueError(f"token ids must be a [batch, steps] tensor of whole numbers, not {list(ids.shape)} of {ids.dtype}")
+        steps = torch.arange(1, ids.shape[1] + 1, device=ids.device)
+        lengths = ((ids >= 0) * steps).amax(1) if ids.shape[1] else torch.zeros(ids.shape[0], dtype=torch.int64, device=ids.device)
+        e = seq.embedding(ids, self.table, math.sqrt(self.width))
+        x, z = self.inputs(e).chunk(2, dim=-1)
+        u = seq.causal_conv(x, self.conv_weight, self.conv_bias, lengths=lengths)
+        dt, a, b, c = self._select(u)
+        y = seq.selective_scan(u, dt, a, b, c, self.skip, z, self.dt_bias, lengths=lengths)
+        return y.sum(1) / lengths.clamp(min=1).unsqueeze(1)
+
+    def start(self, batch: int) -> SequenceState:
+        """The state in front of the first token of `batch` rows, for `step`."""
+        dev = self.table.device
+        return SequenceState(torch.zeros(batch, self.taps - 1, self.width, device=dev), torch.zeros(batch, self.width, self.states, device=dev),
+                             torch.zeros(batch, self.width, device=dev), torch.zeros(batch, 1, device=dev))
+
+    @torch.no_grad()
+    def step(self, ids: Tensor, state: SequenceState) -> Tensor:
+        """One more token [batch] for every row: the features of the rows so far, as `forward` gives them for the whole rows.  `state`
+        moves on in place.  No gradient."""
+        x, z = self.inputs(seq.embedding(ids, self.table, math.sqrt(self.width))).chunk(2, dim=-1)
+        u = seq.causal_conv_step(x, self.conv_weight, self.conv_bias, state=state.conv)
+        dt, a, b, c = self._select(u)
+        state.total.add_(seq.selective_scan_step(u, dt, a, b, c, self.skip, z, self.dt_bias, state=state.scan))
+        state.count.add_(1)
+        return state.total / state.count
+
+
+class SequenceEncoder(MLPEncoder):
+    """An MLPEncoder over a token sequence: `front` (SequenceFeatures) makes `width` features of ids [batch, steps], the MLP and the
+    state update follow as in MLPEncoder.  MultiModN trains both: the chain kernels hand back the features' gradient, `front`'s own
+    kernels take it from there.  The reference's recurrent encoders (rnn_encoder.py, lstm_encoder.py) are torch modules over tabular
+    input; a sequence modality has no counterpart there."""
+
+    def __init__(self, state_size: int, vocabulary: int, width: int, hidden_layers: Tuple[int, ...], activation: Callable = F.relu,
+                 states: int = 16, taps: int = 4, rank: Optional[int] = None, device: Optional[torch.device] = None):
+        if not hidden_layers:
+            raise ValueError("SequenceEncoder needs at least one hidden layer")
+        super().__init__(state_size, width, hidden_layers, activation, device)
+        self.front = SequenceFeatures(vocabulary, width, states, taps, rank, device)
+
+    def forward(self, state: Tensor, x: Tensor) -> Tensor:
+        """x: ids, or (floating) the features themselves."""
+        return super().forward(state, x if x.is_floating_point() else self.front(x))

@@ -19,7 +19,7 @@ import torch.nn.functional as F
 
 from . import hip
 from .decoders import ClassDecoder, MLPDecoder
-from .encoders import MIMIC_MLPEncoder, MLPEncoder, _identity
+from .encoders import MIMIC_MLPEncoder, MLPEncoder, SequenceEncoder, _identity
 from .state import TrainableInitState
 
 
@@ -133,8 +133,10 @@ class HipChainEngine:
                 f"(torch device 'cuda' on ROCm). There is no CPU fallback.")
         self.device = dev
         self._dev_index = dev.index if dev.index is not None else torch.cuda.current_device()
-        self.params: List[torch.nn.Parameter] = list(model.parameters())
-        self.names: List[str] = [n for n, _ in model.named_parameters()]
+        # (what is in front of the chain - a SequenceEncoder's features - keeps its own parameters and gradients)
+        fronts = {id(p) for enc in model.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters()}
+        self.params: List[torch.nn.Parameter] = [p for p in model.parameters() if id(p) not in fronts]
+        self.names: List[str] = [n for n, p in model.named_parameters() if id(p) not in fronts]
         for p in self.params:
             if p.dtype != torch.float32:
                 raise UnsupportedModelError("parameters must be float32")
@@ -1142,6 +1144,18 @@ class HipChainEngine:
     def executed_rows(self) -> List[bool]:
         """Which state rows the last step produced (synchronises; the device NaN policy needs it)."""
         return [bool(v) for v in self.debug_tensor(4, 0, 1, self.E + 1).view(torch.int32).flatten().tolist()]
+
+    def input_grad(self, e: int, batch: int) -> torch.Tensor:
+        """[batch, n_features] gradient of the last training step's loss with respect to encoder e's input (an MLPEncoder with hidden
+        layers that ran in that step): its first hidden layer's pre-activation gradients times that layer's weight."""
+        lin = self.model.encoders[e].layers[0]
+        dpre = self.lib.mmn_debug_buffer(self._plan, 7, e * hip.MAX_LAYERS)
+        if not dpre:
+            raise IndexError(e)
+        dx = torch.empty(batch, lin.in_features, dtype=torch.float32, device=self.device)
+        hip.check(self.lib.mmn_seq_input_grad(dpre, lin.weight.data_ptr(), dx.data_ptr(), batch, lin.out_features, lin.in_features,
+                                              self._stream()), "mmn_seq_input_grad")
+        return dx
 
     def debug_tensor(self, kind: int, index: int, rows: int, cols: int) -> torch.Tensor:
         ptr = self.lib.mmn_debug_buffer(self._plan, kind, index)

@@ -45,7 +45,7 @@ ABI_SYMBOLS = (
 #: every symbol include/mmn_sequence.h declares
 SEQUENCE_SYMBOLS = (
     "mmn_seq_embed", "mmn_seq_embed_grad_bytes", "mmn_seq_embed_grad", "mmn_seq_conv", "mmn_seq_conv_grad_bytes", "mmn_seq_conv_grad",
-    "mmn_seq_conv_step", "mmn_seq_scan_marks", "mmn_seq_scan_bytes", "mmn_seq_scan", "mmn_seq_scan_grad", "mmn_seq_scan_step",
+    "mmn_seq_conv_step", "mmn_seq_scan_marks", "mmn_seq_scan_bytes", "mmn_seq_scan", "mmn_seq_scan_grad", "mmn_seq_scan_step", "mmn_seq_input_grad",
 )
 
 
@@ -255,7 +255,8 @@ def load(path: Optional[str] = None) -> C.CDLL:
             ("mmn_seq_embed_grad", i32, [vp, i32, vp, vp, i64, i64, i32, i32, f32, vp, size, vp]),
             ("mmn_seq_conv", i32, [conv, vp]), ("mmn_seq_conv_grad_bytes", size, [conv]), ("mmn_seq_conv_grad", i32, [conv, vp, size, vp]),
             ("mmn_seq_conv_step", i32, [conv, vp]), ("mmn_seq_scan_marks", size, [scan]), ("mmn_seq_scan_bytes", size, [scan, i32]),
-            ("mmn_seq_scan", i32, [scan, vp, size, vp]), ("mmn_seq_scan_grad", i32, [scan, vp, size, vp]), ("mmn_seq_scan_step", i32, [scan, vp])):
+            ("mmn_seq_scan", i32, [scan, vp, size, vp]), ("mmn_seq_scan_grad", i32, [scan, vp, size, vp]), ("mmn_seq_scan_step", i32, [scan, vp]),
+            ("mmn_seq_input_grad", i32, [vp, vp, vp, i64, i32, i32, vp])):
         getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
     if lib.mmn_version() != VERSION:
         raise MmnError(f"{p}: ABI version {lib.mmn_version()} != expected {VERSION}; rebuild")

@@ -25,8 +25,8 @@ import ctypes as C
 
 from . import hip
 from .decoders import MultiModDecoder
-from .encoders import MultiModEncoder
-from .engine import HipChainEngine, check_criterion
+from .encoders import MultiModEncoder, SequenceEncoder
+from .engine import HipChainEngine, UnsupportedModelError, check_criterion
 from .history import HistoryList, MultiModNHistory, PendingEpoch
 from .metrics import compute_metrics, get_performance_metrics      # noqa: F401  (importable from here as from multimodn/multimodn.py)
 from .state import InitState, TrainableInitState
@@ -260,6 +260,7 @@ class MultiModN(nn.Module):
         state["_dp_world"] = 1
         state["_dp_rank"] = 0
         state["_stager"] = None
+        state.pop("_front_grad_buf", None)
         return state
 
     # ------------------------------------------------------------------------------------------
@@ -537,9 +538,103 @@ class MultiModN(nn.Module):
             return list(eng.executed_rows()[1:])
         return st.executed
 
+    # ------------------------------------------------------------------------------------------ sequence encoders
+    def _has_sequences(self) -> bool:
+        return any(isinstance(e, SequenceEncoder) for e in self.encoders)
+
+    def _check_sequences(self) -> None:
+        if self.per_sample or self._dp_group is not None:
+            raise UnsupportedModelError("models with a SequenceEncoder run neither in per-sample mode nor data parallel")
+
+    def _slot_features(self, data: Sequence[Tensor], pairs) -> Dict[int, Tensor]:
+        """{data slot: features} of the slots that feed a SequenceEncoder token ids (a floating slot holds its features already)."""
+        out: Dict[int, Tensor] = {}
+        for k, e in pairs:
+            enc = self.encoders[e]
+            if isinstance(enc, SequenceEncoder) and not data[k].is_floating_point():
+                out[k] = enc.front(data[k].to(self.device))
+        return out
+
+    def _with_features(self, data: Sequence[Tensor], encoder_sequence) -> List[Tensor]:
+        """`data` with the features in the place of token ids, for the forward-only entry points."""
+        if not self._has_sequences():
+            return data
+        self._check_sequences()
+        with torch.no_grad():
+            found = self._slot_features(data, self.get_encoder_iterable(encoder_sequence, False, train=False))
+        return [found[k] if k in found else t.to(self.device) for k, t in enumerate(data)]
+
+    def _front_grads(self) -> None:
+        """Every front parameter's .grad at its own, zeroed place of one buffer: the backward adds into it, and an optimizer sees the same
+        addresses in every step."""
+        params = [p for enc in self.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters() if p.requires_grad]
+        buf = self.__dict__.get("_front_grad_buf")
+        sig = tuple((id(p), tuple(p.shape), p.device) for p in params)
+        if buf is None or buf[0] != sig:
+            sizes = [(p.numel() + 3) // 4 * 4 for p in params]               # (16-byte places)
+            flat = torch.zeros(sum(sizes), dtype=torch.float32, device=self.device)
+            views, at = [], 0
+            for p, n in zip(params, sizes):
+                views.append(flat[at:at + p.numel()].view(p.shape))
+                at += n
+            buf = self.__dict__["_front_grad_buf"] = (sig, flat, views)
+        buf[1].zero_()
+        for p, g in zip(params, buf[2]):
+            p.grad = g
+
+    def _train_steps_sequences(self, train_loader, optimizer, log_interval=None, logger=None):
+        """The batch loop of train_epoch for models with a SequenceEncoder: the features are made with the step's own parameters, the
+        chain step runs on them as on any batch, and the gradient it leaves at those encoders' inputs goes back through the fronts.
+        One step at a time, NaN skips decided on the host (features of token ids are finite: only other slots can skip)."""
+        self._check_sequences()
+        n_batches = len(train_loader) if hasattr(train_loader, "__len__") else None
+        alpha, beta = float(self.err_penalty), float(self.state_change_penalty)
+        eng, steps = None, 0
+        for batch in train_loader:
+            data, target, encoder_sequence = (list(batch) + [None])[:3]
+            pairs = self.get_encoder_iterable(encoder_sequence, self.shuffle_mode, train=True)
+            rows = int(target.shape[0])
+            if eng is None:
+                eng = self._get_engine(rows)
+                eng.epoch_reset()
+                eng.begin_sequence()
+            else:
+                eng.ensure(rows)
+            optimizer.zero_grad()
+            with torch.enable_grad():
+                features = self._slot_features(data, pairs)
+            inputs = [features[k].detach() if k in features else t.to(self.device) for k, t in enumerate(data)]
+            xs, y, exec_pairs, executed, _ = self._ingest(inputs, target, pairs, "host")
+            b = eng.make_batch(xs, y, exec_pairs, batch_global=rows, device_nan_flags=False)
+            masks = eng.draw_dropout_masks(b, self.dropout_mask_provider) if eng.dropout_encoders else None
+            eng.local_step(b, alpha, beta, accumulate=True)
+            self.__dict__["train_steps_launched"] = self.__dict__.get("train_steps_launched", 0) + 1
+            self._front_grads()
+            ran = {k for k, _ in exec_pairs}
+            for k, e in pairs:
+                if k in features and k in ran and features[k].requires_grad:
+                    features[k].backward(eng.input_grad(e, rows))
+            made = {e for k, e in pairs if k in features and k in ran}
+            for e, enc in enumerate(self.encoders):         # (a front that did not run has no gradient, as in the chain)
+                if isinstance(enc, SequenceEncoder) and e not in made:
+                    for p in enc.front.parameters():
+                        p.grad = None
+            eng.assign_grads(executed)
+            optimizer.step()
+            del masks, xs, y
+            steps += 1
+            if log_interval and (steps - 1) % log_interval == log_interval - 1:
+                v = eng.step_values()
+                logger(f"Batch {steps}/{n_batches}\n"
+                       f"\tLoss: {float(v['loss']):.4f}\n"
+                       f"\tErr loss: {float(v['global_err']):.4f}\n"
+                       f"\tState change: {float(v['global_sc']):.4f}")
+        return eng, steps
+
     def _run_step(self, eng, data, target, encoder_sequence, train: bool, batch_global: Optional[int] = None,
                   optimizer=None):
         """One step on its own (no look-ahead): what test() / the parity tests / smoke() drive."""
+        data = self._with_features(data, encoder_sequence)
         mode = self._nan_mode(eng, optimizer, train)
         st = self._make_step(data, target, encoder_sequence, mode, train)
         if batch_global:
@@ -1200,7 +1295,9 @@ class MultiModN(nn.Module):
             logger = print
         self.train()
         n_batches = len(train_loader)
-        if self.per_sample:
+        if self._has_sequences():
+            eng, _ = self._train_steps_sequences(train_loader, optimizer, log_interval, logger)
+        elif self.per_sample:
             eng = self._train_steps_per_sample(train_loader, optimizer)
         else:
             eng, _ = self._train_steps(train_loader, optimizer, log_interval, logger)
@@ -1261,6 +1358,8 @@ class MultiModN(nn.Module):
         (get_performance_metrics, multimodn.py:22-49) on the decoder fed with the state after the
         last encoder, computed natively (multimodn_amd/metrics.py) instead of via torchmetrics."""
         check_criterion(criterion)
+        if self._has_sequences():
+            self._check_sequences()
         if log_results and not logger:
             logger = print
         self.eval()
@@ -1410,6 +1509,7 @@ class MultiModN(nn.Module):
         As in the reference there is NO NaN skip on this path, and rows of encoders that are not in
         the sequence stay 0."""
         self.eval()
+        x = self._with_features(x, None if encoder_sequence is None else np.asarray(encoder_sequence))
         n_samples = int(x[0].shape[0])
         full = np.zeros((len(self.encoders) + 1, len(self.decoders), n_samples))
         if n_samples == 0:
@@ -1475,6 +1575,8 @@ class MultiModN(nn.Module):
         for i, enc in enumerate(self.encoders):
             print('Encoder {}:'.format(i))
             x = torch.as_tensor(np.asarray(input[i], dtype=np.float32)).reshape(1, -1)
+            if isinstance(enc, SequenceEncoder):            # (its front runs on the GPU only: the table is of what follows it)
+                x = torch.zeros(1, enc.n_features)
             table(enc, (torch.zeros(1, S), x))
             print()
         for i, dec in enumerate(self.decoders):
@@ -1488,6 +1590,7 @@ class MultiModN(nn.Module):
         batch_states: List[Tensor] = []
         for batch in data_loader:
             data, _, encoder_sequence = (list(batch) + [None])[:3]
+            data = self._with_features(data, encoder_sequence)
             n = int(data[0].shape[0])
             eng = self._get_engine(n)
             if not batch_states:

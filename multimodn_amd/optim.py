@@ -78,7 +78,8 @@ class Adam(Optimizer):
             cur_p.clear()
             cur_g.clear()
 
-        for p in params:
+        # (by address: an engine's parameters are neighbours in its flat buffer also where the group lists others between them)
+        for p in sorted(params, key=lambda q: q.data_ptr()):
             g = p.grad if p.grad is not None else last_g.get(id(p))
             if g is None:
                 raise RuntimeError("first optimizer.step(): every parameter needs a gradient buffer "

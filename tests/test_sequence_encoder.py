@@ -1,0 +1,216 @@
+"""SequenceEncoder: a token modality in MultiModN, its features' kernels trained through the fusion chain."""
+import copy
+import math
+import pickle
+
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+import multimodn_amd as mm
+from helpers import rel_err
+from multimodn_amd import hip
+
+gpu = pytest.mark.gpu
+S, V, WIDTH, STEPS, ROWS = 20, 30, 24, 12, 16
+
+
+def build(device="cuda", seed=0, taps=4, states=8, dropout_free=True):
+    torch.manual_seed(seed)
+    encoders = [mm.SequenceEncoder(S, V, WIDTH, (16,), states=states, taps=taps, rank=3), mm.MLPEncoder(S, 6, (8, 8)),
+                mm.SequenceEncoder(S, V + 5, 8, (5, 7), torch.sigmoid, states=4, rank=2)]
+    model = mm.MultiModN(S, encoders, [mm.LogisticDecoder(S), mm.LogisticDecoder(S)], 0.7, 0.4, device=torch.device(device))
+    return model
+
+
+def batch(seed=1, rows=ROWS):
+    g = torch.Generator().manual_seed(seed)
+    a, b = torch.randint(0, V, (rows, STEPS), generator=g), torch.randint(-1, V + 5, (rows, 5), generator=g)
+    ends = torch.randint(0, STEPS + 1, (rows,), generator=g)
+    ends[0], ends[1] = 0, STEPS
+    a[torch.arange(STEPS) >= ends[:, None]] = -1
+    return [a, torch.randn(rows, 6, generator=g), b], torch.randint(0, 2, (rows, 2), generator=g)
+
+
+# ---- the same in 64 bits, step after step on the CPU
+def plain_features(front, ids):
+    out = []
+    silu = F.silu
+    for row in ids:
+        n = int(((row >= 0) * torch.arange(1, len(row) + 1)).max())
+        e = torch.stack([front.table[t] * math.sqrt(front.width) if t >= 0 else torch.zeros_like(front.table[0]) for t in row[:n]]) if n else None
+        total = torch.zeros(front.width, dtype=torch.float64)
+        if n:
+            x, z = (e @ front.inputs.weight.t()).chunk(2, -1)
+            line = torch.cat([torch.zeros(front.taps - 1, front.width, dtype=torch.float64), x])
+            h = torch.zeros(front.width, front.states, dtype=torch.float64)
+            a = -torch.exp(front.a_log)
+            for t in range(n):
+                u = silu(front.conv_bias + (front.conv_weight.t() * line[t:t + front.taps]).sum(0))
+                dt, b, c = (front.select.weight @ u).split((front.rank, front.states, front.states))
+                dt = F.softplus(front.spread.weight @ dt + front.dt_bias)
+                h = torch.exp(dt[:, None] * a) * h + (dt * u)[:, None] * b
+                total = total + ((h * c).sum(-1) + front.skip * u) * silu(z[t])
+        out.append(total / max(n, 1))
+    return torch.stack(out)
+
+
+def plain_step(model, data, y):
+    """(loss, err_loss grid) of the training step (multimodn/multimodn.py:137-202)."""
+    state = model.init_state.state_value.expand(len(y), -1)
+    grid, change = [], 0.0
+
+    def errors(s):
+        return torch.stack([F.cross_entropy(torch.sigmoid(d.fc(s)), y[:, i]) for i, d in enumerate(model.decoders)])
+
+    grid.append(errors(state))
+    for enc, x in zip(model.encoders, data):
+        old = state
+        state = mm.MLPEncoder.forward(enc, state, plain_features(enc.front, x) if isinstance(enc, mm.SequenceEncoder) else x.double())
+        change = change + ((state - old) ** 2).mean()
+        grid.append(errors(state))
+    grid = torch.stack(grid)
+    return grid.mean() * model.err_penalty + change / len(model.encoders) * model.state_change_penalty, grid
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["hip", "torch"])
+def test_training_step_against_64_bits(kind):
+    """Gradients of every parameter, fronts and chain, and the weights after one Adam step.  A gradient sums at most ROWS * STEPS
+    contributions (192), each off by some 3 * STEPS + 60 roundings of terms not over 8 times the largest sum: 300 * 2^-24 * 8 < 1.5e-4."""
+    model = build()
+    wide = copy.deepcopy(model).cpu().double()
+    data, y = batch()
+    opt = mm.optim.Adam(model.parameters(), 1e-2) if kind == "hip" else torch.optim.Adam(model.parameters(), 1e-2)
+    hist = mm.MultiModNHistory(["a", "b"])
+    before = {n: p.detach().clone() for n, p in model.named_parameters()}
+    model.train_epoch([(data, y)], opt, torch.nn.CrossEntropyLoss(), hist)
+    loss, grid = plain_step(wide, data, y)
+    assert rel_err(hist.loss["train"][0], grid.detach().numpy()) < 1e-5
+    grads = dict(zip((n for n, _ in wide.named_parameters()), torch.autograd.grad(loss, list(wide.parameters()))))
+    for n, p in model.named_parameters():
+        assert rel_err(p.grad.cpu().numpy(), grads[n].numpy()) < 1.5e-4, n
+        # Adam's first step is lr * g / (|g| + 1e-8), whose slope is 1e-8 / (|g| + 1e-8)^2: an error of d = 1.5e-4 G (G the largest) moves it
+        # by at most d times the slope at |g| - d, and by 2 at most; the weight's own rounding (2^-24 of a weight under 4) is 2.4e-7
+        g, moved = grads[n], (p.detach() - before[n]).cpu().double()
+        d = 1.5e-4 * g.abs().max()
+        allowed = 1e-2 * (d * 1e-8 / ((g.abs() - d).clamp(min=0) + 1e-8) ** 2).clamp(max=2.0) + 3e-7
+        assert ((moved + 1e-2 * g / (g.abs() + 1e-8)).abs() <= allowed).all(), n
+
+
+@gpu
+def test_training_goes_on_and_entry_points_agree():
+    model = build(seed=3)
+    opt = mm.optim.Adam(model.parameters(), 3e-3)
+    crit = torch.nn.CrossEntropyLoss()
+    batches = [batch(s, rows) for s, rows in ((1, 16), (2, 33), (3, 7))]
+    hist = mm.MultiModNHistory(["a", "b"])
+    grads = None
+    for _ in range(3):
+        model.train_epoch(batches, opt, crit, hist)
+        now = [p.grad.data_ptr() for p in model.parameters()]
+        fronts = [p.grad.data_ptr() for e in model.encoders if isinstance(e, mm.SequenceEncoder) for p in e.front.parameters()]
+        assert grads is None or fronts == grads
+        grads = fronts
+        assert len(set(now)) == len(now)
+    assert np.isfinite(np.array(hist.loss["train"])).all()
+    # the same data with the features in the place of the ids gives the same results
+    data, y = batches[1]
+    with torch.no_grad():
+        feats = [e.front(x.cuda()) if isinstance(e, mm.SequenceEncoder) else x.cuda() for e, x in zip(model.encoders, data)]
+    assert np.array_equal(model.predict(data), model.predict(feats))
+    for p, q in zip(model.get_states([(data, y)]), model.get_states([(feats, y.cuda())])):
+        assert torch.equal(p, q)
+    one, two = model.test([(data, y)], crit), model.test([(feats, y.cuda())], crit)
+    assert all(torch.equal(torch.as_tensor(a), torch.as_tensor(b)) or (torch.as_tensor(a) != torch.as_tensor(a)).all()
+               for r, s in zip(one, two) for a, b in zip(r, s))
+    again = pickle.loads(pickle.dumps(model))
+    assert np.array_equal(again.predict(data), model.predict(data))
+
+
+@gpu
+def test_encoder_sequence_and_slots_of_features():
+    """A slot that holds features trains the chain and leaves its front alone; an encoder outside the sequence has no gradient."""
+    model = build(seed=4)
+    opt = torch.optim.SGD(model.parameters(), 1e-2)
+    data, y = batch(5)
+    feats = model.encoders[2].front(data[2].cuda()).detach().cpu()
+    model.train_epoch([([data[0], data[1], feats], y)], opt, torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[2].front.parameters())
+    assert all(p.grad is not None and p.grad.abs().max() > 0 for p in model.encoders[0].front.parameters())
+    seq = torch.tensor([[2, 1]]).expand(ROWS, -1)
+    model.train_epoch([([data[2], data[1]], y, seq)], opt, torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[0].front.parameters())
+    assert all(p.grad is not None for p in model.encoders[2].front.parameters())
+
+
+@gpu
+def test_missing_values_in_another_slot():
+    """A NaN batch of the tabular modality skips its encoder; the sequence encoders train."""
+    model = build(seed=6)
+    opt = torch.optim.SGD(model.parameters(), 1e-2)
+    data, y = batch(7)
+    data[1][3, 2] = float("nan")
+    model.train_epoch([(data, y)], opt, torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[1].parameters())
+    assert all(torch.isfinite(p.grad).all() for e in (0, 2) for p in model.encoders[e].parameters())
+
+
+@gpu
+def test_features_token_by_token():
+    """step() after the n-th token = forward() of the first n tokens.  Both round each step's states and outputs alike but the projections are
+    other products of the library: 32 bits, sums of 24 terms, 12 steps: under 200 roundings, terms up to 8 times the largest feature."""
+    model = build(seed=8)
+    front = model.encoders[0].front
+    ids = torch.randint(0, V, (5, STEPS), generator=torch.Generator().manual_seed(9)).cuda()
+    ids[2, 3] = -1                                                            # a step without a token
+    state = front.start(5)
+    for t in range(STEPS):
+        got = front.step(ids[:, t], state)
+        with torch.no_grad():
+            want = front(ids[:, :t + 1])
+        rows = [0, 1, 3, 4] if t == 3 else slice(None)                        # (forward: a row ends behind its last token)
+        assert rel_err(got[rows].cpu(), want[rows].cpu()) < 200 * 2.0 ** -24 * 8, t
+
+
+@gpu
+def test_input_gradient():
+    lib = hip.load()
+    g = torch.Generator().manual_seed(10)
+    for rows, hidden, width in ((1, 1, 1), (33, 128, 65), (100, 7, 300), (4096, 32, 64)):
+        d, w = torch.randn(rows, hidden, generator=g).cuda(), torch.randn(hidden, width, generator=g).cuda()
+        dx = torch.empty(rows, width, device="cuda")
+        assert lib.mmn_seq_input_grad(d.data_ptr(), w.data_ptr(), dx.data_ptr(), rows, hidden, width, torch.cuda.current_stream().cuda_stream) == 0
+        want, mag = d.cpu().double() @ w.cpu().double(), d.cpu().double().abs() @ w.cpu().double().abs()
+        assert ((dx.cpu().double() - want).abs() <= (hidden + 1) * 2.0 ** -24 * mag).all()
+    assert lib.mmn_seq_input_grad(d.data_ptr(), w.data_ptr(), dx.data_ptr(), 4, 129, 4, None) == -1
+
+
+# ---- refusals (CPU)
+def test_refusals():
+    with pytest.raises(ValueError):
+        mm.SequenceEncoder(8, 10, 4, ())
+    for bad in (dict(states=0), dict(states=33), dict(taps=5), dict(taps=1)):
+        with pytest.raises(ValueError):
+            mm.SequenceFeatures(10, 4, **bad)
+    front = mm.SequenceFeatures(10, 4)
+    for ids in (torch.zeros(3), torch.zeros(2, 3), torch.zeros(2, 3, 4, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            front(ids)
+    with pytest.raises(hip.MmnError):
+        front(torch.zeros(2, 3, dtype=torch.int64))
+    model = build("cpu")
+    model.per_sample = True
+    data, y = batch()
+    for call in (lambda: model.train_epoch([(data, y)], torch.optim.SGD(model.parameters(), 0.1), torch.nn.CrossEntropyLoss()),
+                 lambda: model.test([(data, y)], torch.nn.CrossEntropyLoss()), lambda: model.predict(data), lambda: model.get_states([(data, y)])):
+        with pytest.raises(mm.UnsupportedModelError):
+            call()
+
+
+def test_encoder_on_features_is_an_mlp_encoder():
+    enc = mm.SequenceEncoder(S, V, WIDTH, (16,))
+    state, x = torch.randn(3, S), torch.randn(3, WIDTH)
+    assert torch.equal(enc(state, x), mm.MLPEncoder.forward(enc, state, x))
+    assert {"front.table", "front.conv_weight", "front.a_log", "layers.0.weight"} <= set(enc.state_dict())
