@@ -20,7 +20,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 struct ScanPlan {
-    int waves, cblocks, seg, nseg, nmark;
+    int waves, cblocks, seg, nseg, nmark, slots;
     int64_t grid;
     bool order;
     size_t off_order, off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
@@ -52,20 +52,24 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), SCAN_SEG) * SCAN_SEG) : (s->steps > 0 ? s->steps : 1);
     p.nseg = s->steps > 0 ? (int)ceil_div(s->steps, p.seg) : 1;
     p.nmark = (int)ceil_div(s->steps, SCAN_CK);
-    p.grid = s->batch * p.nseg * s->groups * p.cblocks;
+    // Backward: rows at a time, the others in turn behind them (8192 waves: eight for each SIMD)
+    const int64_t most = 8192 / ((int64_t)s->groups * tiles);
+    p.slots = (int)(backward && p.nseg == 1 && s->batch > most ? (most > 0 ? most : 1) : s->batch);
+    p.grid = (int64_t)p.slots * p.nseg * s->groups * p.cblocks;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += pad256(n); return o; };
-    const size_t rows = (size_t)s->batch * p.nseg;
-    // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and twice 5.4 for the order, instead of 58 + 175)
-    p.order = s->lengths && p.nseg == 1 && waves >= 896;
+    const size_t rows = (size_t)s->batch * p.nseg, parts = (size_t)p.slots * p.nseg;
+    // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and twice 5.4 for the order, instead of 58 + 175.  Many rows even out by
+    // themselves, one workgroup orders them, and rows taken in turn have to be the same ones in every run.)
+    p.order = s->lengths && p.nseg == 1 && waves >= 896 && s->batch <= 16384 && p.slots == s->batch;
     p.off_order = take(p.order ? sizeof(int32_t) * (size_t)s->batch : 0);
     p.off_segh = take(p.nseg > 1 ? sizeof(float) * rows * s->states * s->width : 0);
     p.off_segdt = take(p.nseg > 1 ? sizeof(float) * rows * s->width : 0);
     p.off_part = p.off_mid = p.off_bc = at;
     if (backward) {
         const int64_t n = (int64_t)(s->states + 2) * s->width;
-        p.off_part = take(sizeof(float) * rows * n);
-        p.off_mid = take(sum_parts_bytes((int64_t)rows, n));
+        p.off_part = take(sizeof(float) * parts * n);
+        p.off_mid = take(sum_parts_bytes((int64_t)parts, n));
         p.off_bc = take(p.cblocks > 1 ? sizeof(float) * (size_t)p.cblocks * s->batch * s->steps * s->groups * 2 * s->states : 0);
     }
     p.bytes = at > 0 ? at : 256;
@@ -96,7 +100,7 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
     a.xb = s->x_row; a.xt = s->x_step; a.dtb = s->dt_row; a.dtt = s->dt_step; a.bb = s->b_row; a.bt = s->b_step; a.bg = s->b_group;
     a.cb = s->c_row; a.ct = s->c_step; a.cg = s->c_group; a.zb = s->z_row; a.zt = s->z_step; a.dyb = s->dy_row; a.dyt = s->dy_step;
     a.steps = s->steps; a.width = s->width; a.groups = s->groups; a.states = s->states; a.softplus = s->softplus;
-    a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.cblocks = p.cblocks;
+    a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.cblocks = p.cblocks; a.slots = p.slots;
     return a;
 }
 
@@ -126,10 +130,12 @@ static int scan_backward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
         else SEQ_LAUNCH((k_scan_link<true, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
     const size_t lds = ScanShape<NP>::grad_lds(p.waves);
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_scan_grad<T, NP>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)ScanShape<NP>::grad_lds(4));
+    const bool many = p.slots < a.batch;
+    const hipError_t e = hipFuncSetAttribute(many ? reinterpret_cast<const void*>(k_scan_grad<T, NP, true>) : reinterpret_cast<const void*>(k_scan_grad<T, NP, false>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)ScanShape<NP>::grad_lds(4));
     if (e != hipSuccess) { mmn_note_hip_error((int)e); return MMN_ERR_HIP; }
-    SEQ_LAUNCH((k_scan_grad<T, NP>), grid, block, lds, st, a);
+    if (many) SEQ_LAUNCH((k_scan_grad<T, NP, true>), grid, block, lds, st, a);
+    else SEQ_LAUNCH((k_scan_grad<T, NP, false>), grid, block, lds, st, a);
     if (p.cblocks > 1) {
         const int64_t rows = a.batch * a.steps * a.groups;
         SEQ_LAUNCH(k_scan_bc<T>, dim3((unsigned)ceil_div(rows * 2 * a.states, 256)), dim3(256), 0, st, a.bc_part, (T*)a.db, (T*)a.dc, rows, a.states, p.cblocks);
@@ -177,7 +183,7 @@ int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, voi
     const ScanArgs a = scan_args(s, p, (char*)ws);
     const int rc = SCAN_TYPES(scan_backward);
     if (rc != MMN_OK) return rc;
-    return sum_parts(a.part, (float*)((char*)ws + p.off_mid), s->dparams, s->batch * p.nseg, (int64_t)(s->states + 2) * s->width, s->width, s->states, st);
+    return sum_parts(a.part, (float*)((char*)ws + p.off_mid), s->dparams, (int64_t)p.slots * p.nseg, (int64_t)(s->states + 2) * s->width, s->width, s->states, st);
 }
 
 int mmn_seq_scan_step(const mmn_seq_scan_desc* s, void* stream) {

@@ -104,12 +104,18 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
     for (int i = 0; i < 2; ++i) { keys[i] = (unsigned*)(w + p.off_keys[i]); pos[i] = (unsigned*)(w + p.off_pos[i]); }
     float* part = (float*)(w + p.off_part);
     const int nwg = rows > 0 ? p.nwg : 0;
+    const bool small = rows > 0 && rows <= SMALL_ROWS && vocab * width <= rows * 16384;   // (a large table is cleared where no id names it only)
     const int64_t clear_wg = ceil_div(vocab, SORT_NT * 8) < 256 ? ceil_div(vocab, SORT_NT * 8) : 256;
     const dim3 hg((unsigned)(nwg + clear_wg)), nt(SORT_NT);
-    if (ids64) SEQ_LAUNCH((k_sort_hist<int64_t, true>), hg, nt, 0, st, (const int64_t*)ids, nullptr, rows, (int)vocab, p.run, nwg, p.bins, 0, hist, present, vocab);
+    if (small) {
+        const int64_t bytes = vocab * width * size, wg = ceil_div(bytes, 16 * SMALL_NT * 4);
+        const dim3 sg(1 + (unsigned)(wg < 1024 ? wg : 1024));
+        if (ids64) SEQ_LAUNCH(k_sort_small<int64_t>, sg, dim3(SMALL_NT), 0, st, (const int64_t*)ids, keys[0], pos[0], (int)rows, (int)vocab, p.bits, p.passes, (char*)out, bytes);
+        else SEQ_LAUNCH(k_sort_small<int32_t>, sg, dim3(SMALL_NT), 0, st, (const int32_t*)ids, keys[0], pos[0], (int)rows, (int)vocab, p.bits, p.passes, (char*)out, bytes);
+    } else if (ids64) SEQ_LAUNCH((k_sort_hist<int64_t, true>), hg, nt, 0, st, (const int64_t*)ids, nullptr, rows, (int)vocab, p.run, nwg, p.bins, 0, hist, present, vocab);
     else SEQ_LAUNCH((k_sort_hist<int32_t, true>), hg, nt, 0, st, (const int32_t*)ids, nullptr, rows, (int)vocab, p.run, nwg, p.bins, 0, hist, present, vocab);
     int at = 0;
-    for (int i = 0; i < p.passes && rows > 0; ++i) {
+    for (int i = 0; i < p.passes && rows > 0 && !small; ++i) {
         if (i == 0) {
             if (ids64) SEQ_LAUNCH((k_sort_pass<int64_t, true>), dim3(nwg), nt, 0, st, (const int64_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, hist, present);
             else SEQ_LAUNCH((k_sort_pass<int32_t, true>), dim3(nwg), nt, 0, st, (const int32_t*)ids, nullptr, nullptr, keys[0], pos[0], rows, (int)vocab, p.run, p.nwg, p.bits, 0, hist, present);
@@ -123,7 +129,7 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
                 : width % (4 / size) == 0 && aligned(grad, 4) && aligned(out, 4) ? 4 / size : 1;
     const int ctiles = (int)ceil_div(width, 64 * v), nchunk = rows > 0 ? p.nchunk : 0;
     const int64_t sumwg = ceil_div((int64_t)nchunk * ctiles, 4);
-    const int64_t zero_wg = ceil_div(vocab, 16) < 2048 ? ceil_div(vocab, 16) : 2048;
+    const int64_t zero_wg = small ? 0 : ceil_div(vocab, 16) < 2048 ? ceil_div(vocab, 16) : 2048;
     if (sumwg + zero_wg > MAX_GRID || ceil_div(width, 64) > 65535) return MMN_ERR_UNSUPPORTED;
     const dim3 sg((unsigned)(sumwg + zero_wg));
 #define SUM(T, V)                                                                                                                \

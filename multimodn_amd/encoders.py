@@ -127,7 +127,9 @@ class SequenceFeatures(nn.Module):
     torch's), forward and backward; there is no CPU fallback.
 
     A row ends behind its last id >= 0: pad with -1.  An id outside the vocabulary inside a row is a step without a token (its
-    embedding is 0).  A row without any token has the features 0."""
+    embedding is 0).  A row without any token has the features 0.  The datasets of this package hand every slot over as float32: the
+    whole numbers there are the ids, and a row with a NaN has NaN features, so that its batch skips the encoder like any
+    other modality's (multimodn/multimodn.py:168)."""
 
     def __init__(self, vocabulary: int, width: int, states: int = 16, taps: int = 4, rank: Optional[int] = None,
                  device: Optional[torch.device] = None):
@@ -152,8 +154,14 @@ class SequenceFeatures(nn.Module):
         return self.spread(dt), -torch.exp(self.a_log), b, c
 
     def forward(self, ids: Tensor) -> Tensor:
-        if ids.dim() != 2 or ids.is_floating_point():
+        if ids.dim() != 2 or ids.is_complex() or ids.dtype == torch.bool:
             raise ValueError(f"token ids must be a [batch, steps] tensor of whole numbers, not {list(ids.shape)} of {ids.dtype}")
+        missing = None
+        if ids.is_floating_point():
+            missing = torch.isnan(ids).any(1, keepdim=True)
+            ids = torch.where(torch.isfinite(ids), ids, -1.0).long()
+        elif ids.dtype not in (torch.int32, torch.int64):
+            ids = ids.long()
         steps = torch.arange(1, ids.shape[1] + 1, device=ids.device)
         lengths = ((ids >= 0) * steps).amax(1) if ids.shape[1] else torch.zeros(ids.shape[0], dtype=torch.int64, device=ids.device)
         e = seq.embedding(ids, self.table, math.sqrt(self.width))
@@ -161,7 +169,8 @@ class SequenceFeatures(nn.Module):
         u = seq.causal_conv(x, self.conv_weight, self.conv_bias, lengths=lengths)
         dt, a, b, c = self._select(u)
         y = seq.selective_scan(u, dt, a, b, c, self.skip, z, self.dt_bias, lengths=lengths)
-        return y.sum(1) / lengths.clamp(min=1).unsqueeze(1)
+        features = y.sum(1) / lengths.clamp(min=1).unsqueeze(1)
+        return features if missing is None else torch.where(missing, math.nan, features)
 
     def start(self, batch: int) -> SequenceState:
         """The state in front of the first token of `batch` rows, for `step`."""
@@ -195,5 +204,5 @@ class SequenceEncoder(MLPEncoder):
         self.front = SequenceFeatures(vocabulary, width, states, taps, rank, device)
 
     def forward(self, state: Tensor, x: Tensor) -> Tensor:
-        """x: ids, or (floating) the features themselves."""
-        return super().forward(state, x if x.is_floating_point() else self.front(x))
+        """x: token ids [batch, steps]"""
+        return super().forward(state, self.front(x))

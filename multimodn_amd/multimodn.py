@@ -25,7 +25,7 @@ import ctypes as C
 
 from . import hip
 from .decoders import MultiModDecoder
-from .encoders import MultiModEncoder, SequenceEncoder
+from .encoders import MLPEncoder, MultiModEncoder, SequenceEncoder
 from .engine import HipChainEngine, UnsupportedModelError, check_criterion
 from .history import HistoryList, MultiModNHistory, PendingEpoch
 from .metrics import compute_metrics, get_performance_metrics      # noqa: F401  (importable from here as from multimodn/multimodn.py)
@@ -547,11 +547,11 @@ class MultiModN(nn.Module):
             raise UnsupportedModelError("models with a SequenceEncoder run neither in per-sample mode nor data parallel")
 
     def _slot_features(self, data: Sequence[Tensor], pairs) -> Dict[int, Tensor]:
-        """{data slot: features} of the slots that feed a SequenceEncoder token ids (a floating slot holds its features already)."""
+        """{data slot: features} of the slots whose token ids feed a SequenceEncoder."""
         out: Dict[int, Tensor] = {}
         for k, e in pairs:
             enc = self.encoders[e]
-            if isinstance(enc, SequenceEncoder) and not data[k].is_floating_point():
+            if isinstance(enc, SequenceEncoder):
                 out[k] = enc.front(data[k].to(self.device))
         return out
 
@@ -585,7 +585,7 @@ class MultiModN(nn.Module):
     def _train_steps_sequences(self, train_loader, optimizer, log_interval=None, logger=None):
         """The batch loop of train_epoch for models with a SequenceEncoder: the features are made with the step's own parameters, the
         chain step runs on them as on any batch, and the gradient it leaves at those encoders' inputs goes back through the fronts.
-        One step at a time, NaN skips decided on the host (features of token ids are finite: only other slots can skip)."""
+        One step at a time, NaN skips decided on the host."""
         self._check_sequences()
         n_batches = len(train_loader) if hasattr(train_loader, "__len__") else None
         alpha, beta = float(self.err_penalty), float(self.state_change_penalty)
@@ -1575,8 +1575,10 @@ class MultiModN(nn.Module):
         for i, enc in enumerate(self.encoders):
             print('Encoder {}:'.format(i))
             x = torch.as_tensor(np.asarray(input[i], dtype=np.float32)).reshape(1, -1)
-            if isinstance(enc, SequenceEncoder):            # (its front runs on the GPU only: the table is of what follows it)
-                x = torch.zeros(1, enc.n_features)
+            if isinstance(enc, SequenceEncoder):            # (its front runs on the GPU only: the table is of the MLP behind it)
+                mlp = MLPEncoder(S, enc.n_features, enc.hidden_layers, enc.activation)
+                mlp.layers = enc.layers
+                enc, x = mlp, torch.zeros(1, enc.n_features)
             table(enc, (torch.zeros(1, S), x))
             print()
         for i, dec in enumerate(self.decoders):

@@ -159,7 +159,8 @@ SCAN = [  # batch, steps, width, groups, states, lengths, state, z, d, dt_bias, 
     (3, 33, 64, 1, 16, [33, 32, 1], False, True, True, True, True), (2, 70, 130, 1, 16, [70, 37], True, True, True, True, True),
     (1, 129, 72, 3, 8, None, True, True, False, True, True), (2, 64, 320, 2, 20, [64, 40], True, True, True, True, True),
     (2, 40, 66, 1, 32, None, True, False, True, False, True), (1, 200, 300, 1, 4, [150], False, True, True, True, False),
-    (40, 9, 65, 1, 16, None, True, True, True, True, True), (2, 48, 560, 1, 5, [-3, 1000], False, True, True, True, True),
+    (40, 9, 65, 1, 16, None, True, True, True, True, True), (1100, 3, 70, 1, 5, "ragged", True, True, True, True, True),
+    (2100, 2, 36, 6, 8, None, False, True, True, True, True), (2, 48, 560, 1, 5, [-3, 1000], False, True, True, True, True),
 ]
 
 
@@ -172,7 +173,7 @@ def scan_case(case, dtype, seed=7):
     return dict(x=normal(g, B, L, 2 * D, dtype=dtype)[..., D:], dt=dt, a=-(torch.rand(D, N, generator=g) * N + 0.05).cuda(), b=b, c=c,
                 d=normal(g, D) if d else None, z=normal(g, B, L, D, dtype=dtype) if z else None,
                 dt_bias=(normal(g, D) - 2.5) if dt_bias and softplus else None, softplus=softplus,
-                lengths=torch.tensor(lengths).cuda() if lengths else None, state=normal(g, B, D, N) if state else None), \
+                lengths=(torch.randint(0, L + 1, (B,), generator=rng(seed)) if lengths == "ragged" else torch.tensor(lengths)).cuda() if lengths else None, state=normal(g, B, D, N) if state else None), \
         normal(g, B, L, D, dtype=dtype), normal(g, B, D, N)
 
 
@@ -204,6 +205,32 @@ def test_scan_and_its_gradients(case, dtype):
         O.check(g.state, *want["dstate"], n["one"], "dstate")
     again = seq.selective_scan_grad(dy, saved, ds)
     assert all(torch.equal(p, q) for p, q in zip(g, again) if p is not None)
+
+
+@gpu
+def test_scan_of_more_rows_than_fit_at_once():
+    """A backward workgroup takes several rows in turn (above 8192 waves): every row as in a batch of its own, sums over all of them."""
+    case = (9001, 2, 5, 1, 3, "ragged", True, True, True, True, True)
+    args, dy, ds = scan_case(case, torch.float32)
+    y, state, saved = seq.selective_scan_forward(**args, return_state=True)
+    g = seq.selective_scan_grad(dy, saved, ds)
+    n = scan_terms(case)
+    rows = torch.tensor([0, 1, 700, 5000, 8191, 8192, 8193, 9000])
+    some = {k: (v[rows.cuda()] if k in ("x", "dt", "b", "c", "z", "state", "lengths") else v) for k, v in args.items()}
+    want = O.scan(**some, dy=dy[rows.cuda()], dstate_out=ds[rows.cuda()])
+    for name in ("x", "dt", "b", "c", "z", "state"):
+        O.check(getattr(g, name)[rows.cuda()], *want["dstate" if name == "state" else name], n["one"], "d" + name)
+    # sums over the batch from the kernel's own per-row gradients: of d(dt_bias) directly, of the others by parts of 4500 rows
+    O.check(g.dt_bias, g.dt.double().sum((0, 1)).cpu(), g.dt.double().abs().sum((0, 1)).cpu(), 2 * 9001 + 24, "d(dt_bias)")
+    parts = []
+    for part in (slice(0, 4500), slice(4500, 9001)):
+        cut = {k: (v[part] if k in ("x", "dt", "b", "c", "z", "state", "lengths") else v) for k, v in args.items()}
+        _, _, s = seq.selective_scan_forward(**cut)
+        parts.append(seq.selective_scan_grad(dy[part], s, ds[part]))
+    mag = O.scan(**some, dy=dy[rows.cuda()], dstate_out=ds[rows.cuda()])           # (the size of one row's terms, from eight of them)
+    for name in ("a", "d"):
+        total = sum(getattr(p, name).double().cpu() for p in parts)
+        O.check(getattr(g, name), total, total.abs() + mag[name][1] * 9001 / 8, 64, "d" + name)
 
 
 @gpu
@@ -263,6 +290,80 @@ def test_scan_long_and_wide_agree_with_parts():
     O.check(g.x, *want["x"], n["one"], "dx")
     O.check(g.a, *want["a"], n["all"], "da")
     O.check(g.state, *want["dstate"], n["one"], "dstate")
+
+
+@gpu
+def test_layouts():
+    """Time-major, expanded, transposed and sliced inputs give what their dense copies give."""
+    g = rng(30)
+    B, L, D, N = 3, 10, 20, 6
+    x = normal(g, L, B, D).transpose(0, 1)                                     # time-major
+    dt = normal(g, 1, L, D).expand(B, L, D)                                    # one row's for all
+    z = normal(g, B, 1, D).expand(B, L, D)                                     # steps that share memory
+    b, c = normal(g, B, N, L).transpose(1, 2), normal(g, B, L, 2 * N)[..., ::2]   # states far apart
+    a, d, bias, w = -torch.rand(N, D, generator=g).cuda().t(), normal(g, 2 * D)[::2], normal(g, D), normal(g, 4, D).t()
+    dy = normal(g, B, D, L).transpose(1, 2)
+    s, cs = normal(g, B, N, D).transpose(1, 2), normal(g, B, D, 3).transpose(1, 2)
+    dense = lambda *t: [v.contiguous() for v in t]
+    one = seq.selective_scan_forward(x, dt, a, b, c, d, z, bias, state=s, return_state=True)
+    two = seq.selective_scan_forward(*dense(x, dt, a, b, c, d, z, bias), state=s.contiguous(), return_state=True)
+    assert all(torch.equal(p, q) for p, q in zip(one[:2], two[:2]))
+    assert all(torch.equal(p, q) for p, q in zip(seq.selective_scan_grad(dy, one[2]), seq.selective_scan_grad(dy.contiguous(), two[2])))
+    one = seq.causal_conv(x, w, bias, state=cs, return_state=True) + seq.causal_conv_grad(dy, x, w, bias, state=cs)
+    two = seq.causal_conv(*dense(x, w, bias), state=cs.contiguous(), return_state=True) + seq.causal_conv_grad(*dense(dy, x, w, bias), state=cs.contiguous())
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    step = [x[:, 0], dt[:, 0], a, b[:, 0], c[:, 0], d, z[:, 0], bias]
+    h1, h2 = s.contiguous(), s.contiguous().clone()
+    assert torch.equal(seq.selective_scan_step(*step, state=h1), seq.selective_scan_step(*dense(*step), state=h2)) and torch.equal(h1, h2)
+    c1, c2 = cs.contiguous(), cs.contiguous().clone()
+    assert torch.equal(seq.causal_conv_step(x[:, 0], w, bias, state=c1), seq.causal_conv_step(*dense(x[:, 0], w, bias), state=c2)) and torch.equal(c1, c2)
+    assert torch.equal(seq.embedding_grad(dy, torch.arange(30).view(3, 10).cuda() % 7, 7), seq.embedding_grad(dy.contiguous(), torch.arange(30).view(3, 10).cuda() % 7, 7))
+
+
+@gpu
+@pytest.mark.parametrize("width", [1, 6, 257])
+def test_steps_of_odd_widths(width):
+    g = rng(31)
+    for dtype in TYPES:
+        x, w = normal(g, 9, 2, width, dtype=dtype), normal(g, width, 3)
+        y, end = seq.causal_conv(x, w, activation=None, return_state=True)
+        state = torch.zeros(9, 2, width, dtype=dtype, device="cuda")
+        for t in range(2):
+            assert torch.equal(seq.causal_conv_step(x[:, t], w, state=state, activation=None), y[:, t])
+        assert torch.equal(state, end)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Tensors of over 2^31 elements: the last rows and steps against the same computed on their own."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    rows, width = 70000, 32768
+    table = torch.randn(rows, width, generator=g, device="cuda", dtype=torch.bfloat16)
+    ids = torch.arange(rows, device="cuda").flip(0)
+    out = seq.embedding(ids, table)
+    assert torch.equal(out[-3:], table[:3].flip(0)) and torch.equal(out[:3], table[-3:].flip(0))
+    grad = seq.embedding_grad(out, ids, rows)
+    assert torch.equal(grad[-3:], table[-3:]) and torch.equal(grad[:3], table[:3])
+    del table, out, grad
+    B, L, D = 3, 360000, 2048
+    x = torch.randn(B, L, D, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(D, 4, generator=g, device="cuda")
+    y = seq.causal_conv(x, w)
+    tail = seq.causal_conv(x[-1:, -50:], w, state=x[-1:, -53:-50])
+    assert torch.equal(y[-1:, -50:], tail)
+    # a decay that forgets within a few steps (softplus(5) * 4 = 20: e^-20 a step, 2^-28 of what came before): the end of the last row by itself
+    dt, a = torch.full((1, 1, D), 5.0, device="cuda", dtype=torch.bfloat16).expand(B, L, D).contiguous(), torch.full((D, 1), -4.0, device="cuda")
+    b = torch.randn(B, L, 1, generator=g, device="cuda", dtype=torch.bfloat16)
+    c = torch.ones(B, L, 1, device="cuda", dtype=torch.bfloat16)
+    y, _, saved = seq.selective_scan_forward(x, dt, a, b, c)
+    short = slice(L - 48, L)
+    cut = [t[-1:, short] for t in (x, dt, b, c)]
+    y1, _, saved1 = seq.selective_scan_forward(cut[0], cut[1], a, cut[2], cut[3])
+    assert torch.allclose(y[-1, -40:].float(), y1[0, -40:].float(), rtol=2.0 ** -7, atol=1e-6)
+    g1 = seq.selective_scan_grad(y, saved)
+    g2 = seq.selective_scan_grad(y1, saved1)
+    assert torch.allclose(g1.x[-1, -40:].float(), g2.x[0, -40:].float(), rtol=2.0 ** -6, atol=1e-6)
+    del g1, g2, y, dt
 
 
 # ------------------------------------------------------------------------------------------------------------------ together

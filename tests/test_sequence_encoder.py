@@ -115,34 +115,55 @@ def test_training_goes_on_and_entry_points_agree():
         grads = fronts
         assert len(set(now)) == len(now)
     assert np.isfinite(np.array(hist.loss["train"])).all()
-    # the same data with the features in the place of the ids gives the same results
+    # a model of plain MLPEncoders with the same weights gives the same results on the features
     data, y = batches[1]
     with torch.no_grad():
         feats = [e.front(x.cuda()) if isinstance(e, mm.SequenceEncoder) else x.cuda() for e, x in zip(model.encoders, data)]
-    assert np.array_equal(model.predict(data), model.predict(feats))
-    for p, q in zip(model.get_states([(data, y)]), model.get_states([(feats, y.cuda())])):
+    plain = mm.MultiModN(S, [mm.MLPEncoder(S, e.n_features, e.hidden_layers, e.activation) for e in model.encoders],
+                         [mm.LogisticDecoder(S), mm.LogisticDecoder(S)], 0.7, 0.4, device=torch.device("cuda"))
+    plain.load_state_dict({k: v for k, v in model.state_dict().items() if ".front." not in k})
+    assert np.array_equal(model.predict(data), plain.predict(feats))
+    for p, q in zip(model.get_states([(data, y)]), plain.get_states([(feats, y.cuda())])):
         assert torch.equal(p, q)
-    one, two = model.test([(data, y)], crit), model.test([(feats, y.cuda())], crit)
-    assert all(torch.equal(torch.as_tensor(a), torch.as_tensor(b)) or (torch.as_tensor(a) != torch.as_tensor(a)).all()
-               for r, s in zip(one, two) for a, b in zip(r, s))
+    for r, s in zip(model.test([(data, y)], crit), plain.test([(feats, y.cuda())], crit)):
+        for a, b in zip(r, s):
+            assert torch.allclose(torch.as_tensor(a), torch.as_tensor(b), rtol=0, atol=0, equal_nan=True)
     again = pickle.loads(pickle.dumps(model))
     assert np.array_equal(again.predict(data), model.predict(data))
 
 
 @gpu
-def test_encoder_sequence_and_slots_of_features():
-    """A slot that holds features trains the chain and leaves its front alone; an encoder outside the sequence has no gradient."""
+def test_encoder_sequences():
+    """An encoder outside the sequence has no gradient, front and chain."""
     model = build(seed=4)
     opt = torch.optim.SGD(model.parameters(), 1e-2)
     data, y = batch(5)
-    feats = model.encoders[2].front(data[2].cuda()).detach().cpu()
-    model.train_epoch([([data[0], data[1], feats], y)], opt, torch.nn.CrossEntropyLoss())
-    assert all(p.grad is None for p in model.encoders[2].front.parameters())
-    assert all(p.grad is not None and p.grad.abs().max() > 0 for p in model.encoders[0].front.parameters())
-    seq = torch.tensor([[2, 1]]).expand(ROWS, -1)
-    model.train_epoch([([data[2], data[1]], y, seq)], opt, torch.nn.CrossEntropyLoss())
-    assert all(p.grad is None for p in model.encoders[0].front.parameters())
-    assert all(p.grad is not None for p in model.encoders[2].front.parameters())
+    order = torch.tensor([[2, 1]]).expand(ROWS, -1)
+    model.train_epoch([([data[2], data[1]], y, order)], opt, torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[0].parameters())
+    assert all(p.grad is not None and p.grad.abs().max() > 0 for p in model.encoders[2].front.parameters())
+
+
+@gpu
+def test_ids_from_the_packages_datasets():
+    """PartitionDataset, a stock DataLoader and DeviceResidentLoader hand ids over as float32: the same training as from whole numbers; a NaN
+    skips the encoder."""
+    (a, x, b), y = batch(5, 32)
+    results = []
+    packed = mm.PartitionDataset(torch.cat([a.float(), x, b.float()], 1).numpy(), y.numpy(), [STEPS, 6, 5])
+    loaders = [[([a[i:i + 16], x[i:i + 16], b[i:i + 16]], y[i:i + 16]) for i in (0, 16)], torch.utils.data.DataLoader(packed, 16),
+               mm.DeviceResidentLoader(packed, 16), [([a[i:i + 16].int().cuda(), x[i:i + 16].cuda(), b[i:i + 16].half()], y[i:i + 16]) for i in (0, 16)]]
+    for loader in loaders:
+        model = build(seed=4)
+        model.train_epoch(loader, mm.optim.Adam(model.parameters(), 1e-3), torch.nn.CrossEntropyLoss())
+        results.append([p.detach().clone() for p in model.parameters()])
+    for other in results[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(results[0], other))
+    gone = a.float()
+    gone[3, 0] = float("nan")
+    model.train_epoch([([gone, x, b], y)], torch.optim.SGD(model.parameters(), 1e-2), torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[0].parameters())
+    assert all(torch.isfinite(p.grad).all() for e in (1, 2) for p in model.encoders[e].parameters())
 
 
 @gpu
@@ -195,7 +216,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             mm.SequenceFeatures(10, 4, **bad)
     front = mm.SequenceFeatures(10, 4)
-    for ids in (torch.zeros(3), torch.zeros(2, 3), torch.zeros(2, 3, 4, dtype=torch.int64)):
+    for ids in (torch.zeros(3), torch.zeros(2, 3, dtype=torch.bool), torch.zeros(2, 3, 4, dtype=torch.int64)):
         with pytest.raises(ValueError):
             front(ids)
     with pytest.raises(hip.MmnError):
@@ -209,8 +230,9 @@ def test_refusals():
             call()
 
 
-def test_encoder_on_features_is_an_mlp_encoder():
+def test_state_dict_and_arch(capsys):
     enc = mm.SequenceEncoder(S, V, WIDTH, (16,))
-    state, x = torch.randn(3, S), torch.randn(3, WIDTH)
-    assert torch.equal(enc(state, x), mm.MLPEncoder.forward(enc, state, x))
     assert {"front.table", "front.conv_weight", "front.a_log", "layers.0.weight"} <= set(enc.state_dict())
+    model = build("cpu")
+    model.display_arch([np.zeros(STEPS), np.zeros(6), np.zeros(5)])
+    assert "Encoder 2:" in capsys.readouterr().out
