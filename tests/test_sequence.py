@@ -1,6 +1,6 @@
 """The sequence operators (multimodn_amd.sequence) against their 64-bit statements (sequence_oracle), and what they refuse."""
-import itertools
 import math
+import os
 
 import pytest
 import torch
@@ -418,6 +418,7 @@ def test_together_gradients_against_differences():
 
 
 @gpu
+@pytest.mark.skipif(os.environ.get("MMN_EFENCE", "0") not in ("", "0"), reason="the electric fence's allocator fills new memory, which a capture does not allow")
 def test_together_captured_into_a_graph():
     """Forward and backward captured, replayed several times with eager work between, against the eager result."""
     ids, lengths, leaves = together_inputs()
