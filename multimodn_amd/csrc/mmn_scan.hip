@@ -59,10 +59,10 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += pad256(n); return o; };
     const size_t rows = (size_t)s->batch * p.nseg, parts = (size_t)p.slots * p.nseg;
-    // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and twice 5.4 for the order, instead of 58 + 175.  Many rows even out by
+    // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and 5.4 for the order, instead of 58 + 175.  Many rows even out by
     // themselves, one workgroup orders them, and rows taken in turn have to be the same ones in every run.)
     p.order = s->lengths && p.nseg == 1 && waves >= 896 && s->batch <= 16384 && p.slots == s->batch;
-    p.off_order = take(p.order ? sizeof(int32_t) * (size_t)s->batch : 0);
+    p.off_order = take(p.order && !s->marks ? sizeof(int32_t) * (size_t)s->batch : 0);
     p.off_segh = take(p.nseg > 1 ? sizeof(float) * rows * s->states * s->width : 0);
     p.off_segdt = take(p.nseg > 1 ? sizeof(float) * rows * s->width : 0);
     p.off_part = p.off_mid = p.off_bc = at;
@@ -87,13 +87,16 @@ static bool scan_strides_ok(const mmn_seq_scan_desc* s, bool backward) {
     return s->width <= most && ok(s->x_step) && ok(s->dt_step) && (!s->z || ok(s->z_step)) && (!backward || ok(s->dy_step));
 }
 
+static size_t marks_of(const mmn_seq_scan_desc* s, const ScanPlan& p) { return (size_t)s->batch * p.nmark * s->states * s->width; }
+
 static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* ws) {
     ScanArgs a;
     a.x = s->x; a.dt = s->dt; a.b = s->b; a.c = s->c; a.z = s->z; a.dy = s->dy;
     a.a = s->a; a.d = s->d; a.dt_bias = s->dt_bias; a.state = s->state; a.dstate_out = s->dstate_out; a.lengths = s->lengths;
     a.y = s->y; a.dx = s->dx; a.ddt = s->ddt; a.dz = s->dz; a.db = s->db; a.dc = s->dc;
     a.state_out = s->state_out; a.dstate = s->dstate;
-    a.order = p.order ? (const int32_t*)(ws + p.off_order) : nullptr;
+    // the rows' order lies behind the marks, where a forward pass leaves it for the backward
+    a.order = !p.order ? nullptr : s->marks ? (const int32_t*)(s->marks + marks_of(s, p)) : (const int32_t*)(ws + p.off_order);
     a.seg_h = (float*)(ws + p.off_segh); a.seg_dt = (float*)(ws + p.off_segdt); a.marks = s->marks;
     a.part = (float*)(ws + p.off_part); a.bc_part = (float*)(ws + p.off_bc);
     a.batch = s->batch;
@@ -120,9 +123,8 @@ static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
 }
 
 template <typename T, int NP>
-static int scan_backward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
+static int scan_backward(const ScanArgs& a, const ScanPlan& p, float* mid, float* dparams, hipStream_t st) {
     const dim3 grid((unsigned)p.grid), block(64 * p.waves);
-    if (p.order) SEQ_LAUNCH(k_scan_order, dim3(1), dim3(1024), 0, st, a.lengths, const_cast<int32_t*>(a.order), (int)a.batch, a.steps);
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, true>), grid, block, 0, st, a);
         const int64_t lanes = a.batch * a.states * a.width;
@@ -136,22 +138,30 @@ static int scan_backward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
     if (e != hipSuccess) { mmn_note_hip_error((int)e); return MMN_ERR_HIP; }
     if (many) SEQ_LAUNCH((k_scan_grad<T, NP, true>), grid, block, lds, st, a);
     else SEQ_LAUNCH((k_scan_grad<T, NP, false>), grid, block, lds, st, a);
-    if (p.cblocks > 1) {
-        const int64_t rows = a.batch * a.steps * a.groups;
-        SEQ_LAUNCH(k_scan_bc<T>, dim3((unsigned)ceil_div(rows * 2 * a.states, 256)), dim3(256), 0, st, a.bc_part, (T*)a.db, (T*)a.dc, rows, a.states, p.cblocks);
-    }
+    const float* part = a.part;
+    int64_t parts = (int64_t)p.slots * p.nseg;
+    const int64_t n = (int64_t)(a.states + 2) * a.width, rows = a.batch * a.steps * a.groups;
+    const int rc = sum_many_parts(part, parts, mid, n, a.width, st);
+    if (rc != MMN_OK) return rc;
+    const int64_t sum_wg = ceil_div(n, SUM_COLS), bc_wg = p.cblocks > 1 ? ceil_div(rows * 2 * a.states, SUM_NT) : 0;
+    if (sum_wg + bc_wg > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+    SEQ_LAUNCH(k_scan_sums<T>, dim3((unsigned)(sum_wg + bc_wg)), dim3(SUM_NT), 0, st, part, dparams, parts, n, a.width, a.states, (unsigned)sum_wg,
+               a.bc_part, (T*)a.db, (T*)a.dc, rows, a.states, p.cblocks);
     return MMN_OK;
 }
 
-#define SCAN_STATES(FN, T)                                                                                      \
-    (padded_states(s->states) == 4 ? FN<T, 4>(a, p, st) : padded_states(s->states) == 8 ? FN<T, 8>(a, p, st)    \
-     : padded_states(s->states) == 16 ? FN<T, 16>(a, p, st) : FN<T, 32>(a, p, st))
-#define SCAN_TYPES(FN) (s->type == MMN_SEQ_F32 ? SCAN_STATES(FN, float) : s->type == MMN_SEQ_BF16 ? SCAN_STATES(FN, bf16) : SCAN_STATES(FN, f16))
+#define SCAN_STATES(FN, T, ...)                                                                                          \
+    (padded_states(s->states) == 4 ? FN<T, 4>(__VA_ARGS__) : padded_states(s->states) == 8 ? FN<T, 8>(__VA_ARGS__)       \
+     : padded_states(s->states) == 16 ? FN<T, 16>(__VA_ARGS__) : FN<T, 32>(__VA_ARGS__))
+#define SCAN_TYPES(FN, ...)                                                                                              \
+    (s->type == MMN_SEQ_F32 ? SCAN_STATES(FN, float, __VA_ARGS__) : s->type == MMN_SEQ_BF16 ? SCAN_STATES(FN, bf16, __VA_ARGS__) : SCAN_STATES(FN, f16, __VA_ARGS__))
 
 extern "C" {
 
 size_t mmn_seq_scan_marks(const mmn_seq_scan_desc* s) {
-    return scan_sizes_ok(s) ? (size_t)s->batch * scan_plan(s, false).nmark * s->states * s->width : 0;
+    if (!scan_sizes_ok(s)) return 0;
+    const ScanPlan p = scan_plan(s, false);
+    return marks_of(s, p) + (p.order ? (size_t)s->batch : 0);
 }
 
 size_t mmn_seq_scan_bytes(const mmn_seq_scan_desc* s, int backward) { return scan_sizes_ok(s) ? scan_plan(s, backward != 0).bytes : 0; }
@@ -166,7 +176,7 @@ int mmn_seq_scan(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* st
     if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 64) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
     const ScanArgs a = scan_args(s, p, (char*)ws);
-    return SCAN_TYPES(scan_forward);
+    return SCAN_TYPES(scan_forward, a, p, st);
 }
 
 int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, void* stream) {
@@ -175,15 +185,14 @@ int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, voi
     if (!s->a || !s->x || !s->dt || !s->b || !s->c || !s->marks || !s->dy || !s->dx || !s->ddt || !s->db || !s->dc || !s->dparams ||
         (s->z && !s->dz)) return MMN_ERR_ARG;
     if (!scan_strides_ok(s, true)) return MMN_ERR_UNSUPPORTED;
-    const ScanPlan p = scan_plan(s, true);
+    ScanPlan p = scan_plan(s, true);
+    p.order = p.order && scan_plan(s, false).order;
     if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
     if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 64) > MAX_GRID ||
-        ceil_div(s->batch * s->steps * s->groups * 2 * s->states, 256) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
+        ceil_div(s->batch * s->steps * s->groups * 2 * s->states, SUM_NT) > MAX_GRID) return MMN_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
     const ScanArgs a = scan_args(s, p, (char*)ws);
-    const int rc = SCAN_TYPES(scan_backward);
-    if (rc != MMN_OK) return rc;
-    return sum_parts(a.part, (float*)((char*)ws + p.off_mid), s->dparams, (int64_t)p.slots * p.nseg, (int64_t)(s->states + 2) * s->width, s->width, s->states, st);
+    return SCAN_TYPES(scan_backward, a, p, (float*)((char*)ws + p.off_mid), s->dparams, st);
 }
 
 int mmn_seq_scan_step(const mmn_seq_scan_desc* s, void* stream) {
