@@ -22,7 +22,7 @@ static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 
 struct ScanPlan {
     int waves, cblocks, seg, nseg, nmark, slots;
     int64_t grid;
-    bool order;
+    bool sorted, order;     // rows' order is made and kept with the marks; it is used
     size_t off_order, off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
 };
 static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
@@ -61,7 +61,8 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     const size_t rows = (size_t)s->batch * p.nseg, parts = (size_t)p.slots * p.nseg;
     // (4096 rows of up to 48 steps, 64 channels: 46 + 132 us and 5.4 for the order, instead of 58 + 175.  Many rows even out by
     // themselves, one workgroup orders them, and rows taken in turn have to be the same ones in every run.)
-    p.order = s->lengths && p.nseg == 1 && waves >= 896 && s->batch <= 16384 && p.slots == s->batch;
+    p.sorted = s->lengths && s->steps > 0 && waves >= 896 && s->batch <= 16384;       // (by sizes alone: both passes agree on it)
+    p.order = p.sorted && p.nseg == 1 && p.slots == s->batch;
     p.off_order = take(p.order && !s->marks ? sizeof(int32_t) * (size_t)s->batch : 0);
     p.off_segh = take(p.nseg > 1 ? sizeof(float) * rows * s->states * s->width : 0);
     p.off_segdt = take(p.nseg > 1 ? sizeof(float) * rows * s->width : 0);
@@ -87,7 +88,7 @@ static bool scan_strides_ok(const mmn_seq_scan_desc* s, bool backward) {
     return s->width <= most && ok(s->x_step) && ok(s->dt_step) && (!s->z || ok(s->z_step)) && (!backward || ok(s->dy_step));
 }
 
-static size_t marks_of(const mmn_seq_scan_desc* s, const ScanPlan& p) { return (size_t)s->batch * p.nmark * s->states * s->width; }
+template <typename S> static size_t marks_of(const S& s, const ScanPlan& p) { return (size_t)s.batch * p.nmark * s.states * s.width; }
 
 static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* ws) {
     ScanArgs a;
@@ -96,7 +97,7 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
     a.y = s->y; a.dx = s->dx; a.ddt = s->ddt; a.dz = s->dz; a.db = s->db; a.dc = s->dc;
     a.state_out = s->state_out; a.dstate = s->dstate;
     // the rows' order lies behind the marks, where a forward pass leaves it for the backward
-    a.order = !p.order ? nullptr : s->marks ? (const int32_t*)(s->marks + marks_of(s, p)) : (const int32_t*)(ws + p.off_order);
+    a.order = !p.order ? nullptr : s->marks ? (const int32_t*)(s->marks + marks_of(*s, p)) : (const int32_t*)(ws + p.off_order);
     a.seg_h = (float*)(ws + p.off_segh); a.seg_dt = (float*)(ws + p.off_segdt); a.marks = s->marks;
     a.part = (float*)(ws + p.off_part); a.bc_part = (float*)(ws + p.off_bc);
     a.batch = s->batch;
@@ -110,11 +111,15 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
 template <typename T, int NP>
 static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)p.grid), block(64 * p.waves);
-    if (p.order) SEQ_LAUNCH(k_scan_order, dim3(1), dim3(1024), 0, st, a.lengths, const_cast<int32_t*>(a.order), (int)a.batch, a.steps);
+    if (p.sorted && (a.order || a.marks)) {
+        int32_t* order = a.order ? const_cast<int32_t*>(a.order) : (int32_t*)(a.marks + marks_of(a, p));
+        SEQ_LAUNCH(k_scan_order, dim3(1), dim3(1024), 0, st, a.lengths, order, (int)a.batch, a.steps);
+    }
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, false>), grid, block, 0, st, a);
         const int64_t lanes = a.batch * a.states * a.width;
-        if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<false, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
+        if (p.nseg <= LINK_NEAR) {}                          // (the segments themselves: link_near)
+        else if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<false, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
         else SEQ_LAUNCH((k_scan_link<false, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
     if (a.marks) SEQ_LAUNCH((k_scan<T, NP, true>), grid, block, 0, st, a);
@@ -128,7 +133,8 @@ static int scan_backward(const ScanArgs& a, const ScanPlan& p, float* mid, float
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, true>), grid, block, 0, st, a);
         const int64_t lanes = a.batch * a.states * a.width;
-        if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<true, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
+        if (p.nseg <= LINK_NEAR) {}                          // (the segments themselves: link_near)
+        else if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<true, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
         else SEQ_LAUNCH((k_scan_link<true, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
     const size_t lds = ScanShape<NP>::grad_lds(p.waves);
@@ -161,7 +167,7 @@ extern "C" {
 size_t mmn_seq_scan_marks(const mmn_seq_scan_desc* s) {
     if (!scan_sizes_ok(s)) return 0;
     const ScanPlan p = scan_plan(s, false);
-    return marks_of(s, p) + (p.order ? (size_t)s->batch : 0);
+    return marks_of(*s, p) + (p.sorted ? (size_t)s->batch : 0);
 }
 
 size_t mmn_seq_scan_bytes(const mmn_seq_scan_desc* s, int backward) { return scan_sizes_ok(s) ? scan_plan(s, backward != 0).bytes : 0; }
@@ -185,8 +191,7 @@ int mmn_seq_scan_grad(const mmn_seq_scan_desc* s, void* ws, size_t ws_bytes, voi
     if (!s->a || !s->x || !s->dt || !s->b || !s->c || !s->marks || !s->dy || !s->dx || !s->ddt || !s->db || !s->dc || !s->dparams ||
         (s->z && !s->dz)) return MMN_ERR_ARG;
     if (!scan_strides_ok(s, true)) return MMN_ERR_UNSUPPORTED;
-    ScanPlan p = scan_plan(s, true);
-    p.order = p.order && scan_plan(s, false).order;
+    const ScanPlan p = scan_plan(s, true);
     if (!ws || !aligned(ws, 256) || ws_bytes < p.bytes) return MMN_ERR_WORKSPACE;
     if (p.grid > MAX_GRID || ceil_div(s->batch * s->states * s->width, 64) > MAX_GRID ||
         ceil_div(s->batch * s->steps * s->groups * 2 * s->states, SUM_NT) > MAX_GRID) return MMN_ERR_UNSUPPORTED;

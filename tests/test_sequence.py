@@ -321,6 +321,27 @@ def test_layouts():
 
 
 @gpu
+def test_backward_of_another_layout():
+    """A forward pass over x whose steps lie 32 MB apart (rows in segments, for 32-bit offsets), the backward over its dense copy."""
+    case = (900, 48, 6, 1, 4, "ragged", True, True, True, True, True)
+    args, dy, ds = scan_case(case, torch.float32)
+    far = torch.zeros(48, 1 << 23, device="cuda")[:, :6]
+    far.copy_(args["x"][0])
+    args["x"] = far.expand(900, 48, 6)
+    y, state, saved = seq.selective_scan_forward(**args, return_state=True)
+    g = seq.selective_scan_grad(dy, saved._replace(x=args["x"].contiguous()), ds)
+    n = scan_terms(case)
+    rows = torch.tensor([0, 1, 450, 899])
+    some = {k: (v[rows.cuda()] if k in ("x", "dt", "b", "c", "z", "state", "lengths") else v) for k, v in args.items()}
+    want = O.scan(**some, dy=dy[rows.cuda()], dstate_out=ds[rows.cuda()])
+    O.check(y[rows.cuda()], *want["y"], n["y"], "y")
+    for name in ("x", "dt", "b", "c", "z", "state"):
+        O.check(getattr(g, name)[rows.cuda()], *want["dstate" if name == "state" else name], n["one"], "d" + name)
+    for one, two in zip(g, seq.selective_scan_grad(dy, saved, ds)):            # and over the same: in segments
+        assert torch.allclose(one, two, rtol=1e-3, atol=1e-3 * float(one.abs().max()))
+
+
+@gpu
 @pytest.mark.parametrize("width", [1, 6, 257])
 def test_steps_of_odd_widths(width):
     g = rng(31)
