@@ -129,6 +129,14 @@ Tensor state_pair(const Opt& state, const Opt& out_state) {
 void moved(const Tensor& t) {                                        // written through its address: autograd's saved copies are stale
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// Does an autograd graph made on the default stream still hold this leaf?  A backward pass captured on another stream would hand it
+// the gradient there, which no capture allows and ends the process.
+bool held_eagerly(const Opt& t) {
+    if (!t || !t->requires_grad() || !t->is_leaf()) return false;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : c10::nullopt;
+    return stream && stream->id() == 0;
+}
 const void* ptr(const Opt& t) { return t ? t->data_ptr() : nullptr; }
 template <typename T> T* at_of(const Opt& t) { return t ? (T*)t->data_ptr() : nullptr; }
 
@@ -369,6 +377,7 @@ Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tenso
 PYBIND11_MODULE(_binding, m) {
     m.def("bind", &bind);
     m.def("source_hash", [] { return std::string(MMN_SOURCE_HASH); });
+    m.def("held_eagerly", &held_eagerly);
     m.def("embed", &embed);
     m.def("embed_grad", &embed_grad);
     m.def("conv", &conv);

@@ -12,7 +12,8 @@ table) and the scan's states are float32, and so are all sums inside.  Tensors a
 any other strides (anything else is copied); results are dense.  `lengths` ([batch], whole numbers) says how many steps of each row
 count: what stands behind them is not read, gives 0 and leaves the states as they are.  Results do not change from run to run.
 
-Everything runs on the current stream of the tensors' device, may be captured into a graph, and has no CPU or torch-op fallback: off
+Everything runs on the current stream of the tensors' device, may be captured into a graph (with autograd: once no eager graph holds the
+leaves any more; refused before), and has no CPU or torch-op fallback: off
 an AMD GPU these functions raise.  The reference has no counterpart: its recurrent encoders (multimodn/encoders/rnn_encoder.py,
 lstm_encoder.py) are torch modules.
 """
@@ -38,10 +39,18 @@ def _any_grad(*tensors: Optional[Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _check_capture(*tensors: Optional[Tensor]) -> None:
+    """Refuses to record for autograd, inside a graph capture, on a leaf that an eager graph still holds."""
+    if tensors[0].is_cuda and torch.cuda.is_current_stream_capturing() and any(_native().held_eagerly(t) for t in tensors):
+        raise hip.MmnError("an autograd graph made outside this capture still holds one of these leaves: drop its outputs and losses first "
+                           "(the captured backward pass would add to the leaf on the default stream), or call under torch.no_grad()")
+
+
 # ---------------------------------------------------------------------------------------------------------------- embedding
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale):
+        _check_capture(weight)
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.scale = weight.shape[0], scale
         return _native().embed(ids, weight, scale)
@@ -84,6 +93,7 @@ def _silu(activation: Optional[str]) -> bool:
 class _Conv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, activation, lengths, return_state):
+        _check_capture(x, weight, bias, state)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, lengths, state)
         ctx.activation = activation
@@ -156,6 +166,7 @@ class ScanSaved(NamedTuple):
 class _Scan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, return_state):
+        _check_capture(x, dt, a, b, c, d, z, dt_bias, state)
         ctx.set_materialize_grads(False)
         y, out, *saved = _native().scan(x, dt, a, b, c, d, z, dt_bias, softplus, lengths, state, return_state, True)
         ctx.save_for_backward(*saved)

@@ -482,6 +482,52 @@ def test_together_captured_into_a_graph():
 
 
 @gpu
+@pytest.mark.skipif(os.environ.get("MMN_EFENCE", "0") not in ("", "0"), reason="the electric fence's allocator fills new memory, which a capture does not allow")
+def test_autograd_captured_once_no_eager_graph_is_left():
+    """While an eager graph holds a leaf the capture is refused at the first call; afterwards forward and backward replay the eager result."""
+    ids, lengths, leaves = together_inputs()
+    table, w, wb, proj, a, dt_bias, d = [t.clone().requires_grad_(True) for t in leaves]
+    params = [table, w, wb, a, dt_bias, d]
+    dy = normal(rng(13), 3, 14, 16)
+    D, N = a.shape
+    dt, bc = normal(rng(14), 3, 14, D), normal(rng(15), 3, 14, N)
+
+    def run():
+        e = seq.embedding(ids, table, 4.0)
+        u = seq.causal_conv(e, w, wb, lengths=lengths)
+        return seq.selective_scan(u, dt, a, bc, bc, d, e, dt_bias, lengths=lengths)
+
+    y = run()
+    want = [t.clone() for t in torch.autograd.grad(y, params, dy, retain_graph=True)]
+    torch.cuda.synchronize()
+    with pytest.raises(hip.MmnError, match="drop its outputs"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            run()
+    for call in (lambda: seq.causal_conv(dy, w, wb), lambda: seq.selective_scan(dy, dt, a, bc, bc)):
+        with pytest.raises(hip.MmnError, match="drop its outputs"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del y
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(run(), params, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(run(), params, dy)
+    for turn in range(3):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
+        again = torch.autograd.grad(run(), params, dy)
+        assert all(torch.equal(p, q) for p, q in zip(again, want))
+
+
+@gpu
 def test_on_another_stream():
     ids, lengths, leaves = together_inputs()
     table, w, wb, proj, a, dt_bias, d = leaves
