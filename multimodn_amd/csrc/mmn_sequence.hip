@@ -103,6 +103,29 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
     unsigned *keys[2], *pos[2];
     for (int i = 0; i < 2; ++i) { keys[i] = (unsigned*)(w + p.off_keys[i]); pos[i] = (unsigned*)(w + p.off_pos[i]); }
     float* part = (float*)(w + p.off_part);
+    const int v = width % (16 / size) == 0 && aligned(grad, 16) && aligned(out, 16) ? 16 / size
+                : width % (4 / size) == 0 && aligned(grad, 4) && aligned(out, 4) ? 4 / size : 1;
+    // A workgroup of k_embed_few has 256 bytes of its table rows.  It is taken where two workgroups a CU own the table (8192 ids, fp32 rows
+    // of 203: 12 us instead of 27 for a table of 1501 rows, 18 instead of 30 for 8192, 31 and 31 for 16384; where all 8192 ids are
+    // one 36 instead of 19, for its workgroups read them alone).
+    const int fv = size == 2 && width % 2 == 0 && aligned(grad, 4) && aligned(out, 4) ? 2 : 1;
+    const int64_t tiles = ceil_div(width, 64 * fv);
+    if (rows <= FEW_ROWS && vocab * tiles <= 512 * FEW_R) {
+        int nb = 0, bits = 0;
+        while (((int64_t)1 << nb) < vocab && ((tiles << (nb + 1)) <= 512 || ceil_div(vocab, 1 << nb) > FEW_R)) ++nb;
+        while (((int64_t)1 << bits) < ceil_div(vocab, 1 << nb)) ++bits;
+        const dim3 fg((unsigned)(tiles << nb));
+#define FEW(T, V)                                                                                                                \
+    do {                                                                                                                         \
+        if (ids64) SEQ_LAUNCH((k_embed_few<T, int64_t, V>), fg, dim3(FEW_NT), 0, st, (const int64_t*)ids, (const T*)grad, (T*)out, (int)rows, (int)vocab, width, (int)tiles, nb, bits, scale); \
+        else SEQ_LAUNCH((k_embed_few<T, int32_t, V>), fg, dim3(FEW_NT), 0, st, (const int32_t*)ids, (const T*)grad, (T*)out, (int)rows, (int)vocab, width, (int)tiles, nb, bits, scale); \
+    } while (0)
+        if (type == MMN_SEQ_F32) FEW(float, 1);
+        else if (type == MMN_SEQ_BF16) { if (fv == 2) FEW(bf16, 2); else FEW(bf16, 1); }
+        else { if (fv == 2) FEW(f16, 2); else FEW(f16, 1); }
+#undef FEW
+        return MMN_OK;
+    }
     const int nwg = rows > 0 ? p.nwg : 0;
     const bool small = rows > 0 && rows <= SMALL_ROWS && vocab * width <= rows * 16384;   // (a large table is cleared where no id names it only)
     const int64_t clear_wg = ceil_div(vocab, SORT_NT * 8) < 256 ? ceil_div(vocab, SORT_NT * 8) : 256;
@@ -125,8 +148,6 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
             at = 1 - at;
         }
     }
-    const int v = width % (16 / size) == 0 && aligned(grad, 16) && aligned(out, 16) ? 16 / size
-                : width % (4 / size) == 0 && aligned(grad, 4) && aligned(out, 4) ? 4 / size : 1;
     const int ctiles = (int)ceil_div(width, 64 * v), nchunk = rows > 0 ? p.nchunk : 0;
     const int64_t sumwg = ceil_div((int64_t)nchunk * ctiles, 4);
     const int64_t zero_wg = small ? 0 : ceil_div(vocab, 16) < 2048 ? ceil_div(vocab, 16) : 2048;

@@ -23,6 +23,7 @@ def normal(g, *shape, dtype=torch.float32, device="cuda"):
 # ---------------------------------------------------------------------------------------------------------------- embedding
 EMBED = [  # ids shape, vocabulary, width
     ((1,), 1, 1), ((16, 1), 1000, 64), ((5, 7), 11, 3), ((33,), 300, 130), ((2, 3, 4), 70000, 66), ((700,), 5, 513), ((4097,), 2000, 8), ((9000,), 300000, 5), ((0,), 9, 4),
+    ((8192,), 1501, 203), ((64, 128), 64, 64), ((1025,), 8192, 200), ((8193,), 1501, 66), ((5000,), 60000, 9), ((300,), 500, 4225), ((4000,), 40000, 130),
 ]
 
 
@@ -57,6 +58,19 @@ def test_embedding_gradient_of_many_places_and_of_one_token():
         got = seq.embedding_grad(grad, ids.cuda(), vocab, 0.5)
         want, mag, count = O.embed_grad(grad, ids, vocab, 0.5)
         O.check(got, want, mag, (count + 2)[:, None].double(), f"{n} places")
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 63, 1024, 8192, 8193])
+def test_embedding_gradient_of_ids_that_name_no_row(rows):
+    grad = torch.full((rows, 70), float("nan"), device="cuda")
+    for vocab in (3, 700, 60000):
+        assert not seq.embedding_grad(grad, torch.full((rows,), -1, device="cuda"), vocab).any()
+        ids = torch.full((rows,), vocab, device="cuda")
+        ids[rows // 2] = vocab - 1
+        grad[rows // 2] = 1.0
+        got = seq.embedding_grad(grad, ids, vocab, 2.0)
+        assert not got[:-1].any() and torch.equal(got[-1], torch.full((70,), 2.0, device="cuda"))
 
 
 @gpu
