@@ -38,10 +38,10 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     p.cblocks = (int)ceil_div(tiles, p.waves);
     // Segments, each of which costs a first pass over its steps: enough for two waves on each of the 1024 SIMDs (all that fit of the
     // backward kernel), half as many again where rows differ in length (4 rows of up to 2048 steps, 1024 channels: 241 us forward and
-    // backward with 3072 waves, 270 with 2048, 248 with 4096).  From 896 waves on the rows are enough by themselves (512 steps, 64
+    // backward with three waves a SIMD, 270 with two, 248 with four).  From 896 waves on the rows are enough by themselves (512 steps, 64
     // channels, fp32: 600 rows 790 us in segments and 965 in one piece; 1000 rows 1071 and 1045; 1500 rows 1631 and 1511).
     const int64_t waves = s->batch * s->groups * tiles;
-    const int64_t want = waves >= 896 ? 1 : ceil_div(s->lengths ? 3072 : 2048, waves > 0 ? waves : 1);
+    const int64_t want = waves >= 896 ? 1 : ceil_div(1024 * (s->lengths ? 3 : 2), waves > 0 ? waves : 1);
     int64_t n = ceil_div(s->steps, SCAN_SEG);
     n = want < n ? want : n;
     // ... and as many as it takes for a segment of the widest strided tensor to stay below 2^30 bytes (32-bit offsets in the kernels)
