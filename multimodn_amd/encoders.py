@@ -180,8 +180,8 @@ class SequenceFeatures(nn.Module):
 
     @torch.no_grad()
     def step(self, ids: Tensor, state: SequenceState) -> Tensor:
-        """One more token [batch] for every row: the features of the rows so far, as `forward` gives them for the whole rows.  `state`
-        moves on in place.  No gradient."""
+        """One more token [batch] for every row: the features of the rows so far, as `forward` gives them for the whole rows.  An id
+        below 0 is a step without a token here, also at a row's end.  `state` moves on in place.  No gradient."""
         x, z = self.inputs(seq.embedding(ids, self.table, math.sqrt(self.width))).chunk(2, dim=-1)
         u = seq.causal_conv_step(x, self.conv_weight, self.conv_bias, state=state.conv)
         dt, a, b, c = self._select(u)

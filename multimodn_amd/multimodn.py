@@ -545,6 +545,14 @@ class MultiModN(nn.Module):
     def _check_sequences(self) -> None:
         if self.per_sample or self._dp_group is not None:
             raise UnsupportedModelError("models with a SequenceEncoder run neither in per-sample mode nor data parallel")
+        fronts = [e.front for e in self.encoders if isinstance(e, SequenceEncoder)]
+        held = {id(p) for f in fronts for p in f.parameters()}
+        if any(id(p) in held for enc in self.encoders for n, p in enc.named_parameters(remove_duplicate=False)
+               if not (isinstance(enc, SequenceEncoder) and n.startswith("front."))) or \
+                any(id(p) in held for m in (self.decoders, self.init_state) for p in m.parameters()):
+            raise UnsupportedModelError("a SequenceEncoder's front shares no parameter with the chain")
+        if any(p.dtype != torch.float32 for f in fronts for p in f.parameters()):
+            raise UnsupportedModelError("parameters must be float32")
 
     def _slot_features(self, data: Sequence[Tensor], pairs) -> Dict[int, Tensor]:
         """{data slot: features} of the slots whose token ids feed a SequenceEncoder."""
@@ -567,7 +575,8 @@ class MultiModN(nn.Module):
     def _front_grads(self) -> None:
         """Every front parameter's .grad at its own, zeroed place of one buffer: the backward adds into it, and an optimizer sees the same
         addresses in every step."""
-        params = [p for enc in self.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters() if p.requires_grad]
+        params = list({id(p): p for enc in self.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters()
+                       if p.requires_grad}.values())
         buf = self.__dict__.get("_front_grad_buf")
         sig = tuple((id(p), tuple(p.shape), p.device) for p in params)
         if buf is None or buf[0] != sig:
@@ -614,11 +623,12 @@ class MultiModN(nn.Module):
             for k, e in pairs:
                 if k in features and k in ran and features[k].requires_grad:
                     features[k].backward(eng.input_grad(e, rows))
-            made = {e for k, e in pairs if k in features and k in ran}
-            for e, enc in enumerate(self.encoders):         # (a front that did not run has no gradient, as in the chain)
-                if isinstance(enc, SequenceEncoder) and e not in made:
+            made = {id(p) for k, e in pairs if k in features and k in ran for p in self.encoders[e].front.parameters()}
+            for enc in self.encoders:                       # (a front that did not run has no gradient, as in the chain)
+                if isinstance(enc, SequenceEncoder):
                     for p in enc.front.parameters():
-                        p.grad = None
+                        if id(p) not in made:
+                            p.grad = None
             eng.assign_grads(executed)
             optimizer.step()
             del masks, xs, y

@@ -145,6 +145,27 @@ def test_encoder_sequences():
 
 
 @gpu
+def test_fronts_that_share_a_table():
+    """Its gradient is the sum of both encoders' (each sum rounded once: half a step of fp32), or the one's that ran."""
+    def twin(tied, encoders):
+        torch.manual_seed(8)
+        encs = [mm.SequenceEncoder(S, V, WIDTH, (16,), states=8), mm.SequenceEncoder(S, V, WIDTH, (8,), states=4)]
+        encs[1].front.table.data.copy_(encs[0].front.table.data)
+        if tied:
+            encs[1].front.table = encs[0].front.table
+        model = mm.MultiModN(S, encs, [mm.LogisticDecoder(S)], 0.7, 0.4, device=torch.device("cuda"))
+        data, y = batch(5)
+        order = torch.tensor([encoders]).expand(ROWS, -1)
+        model.train_epoch([([data[0]] * len(encoders), y[:, :1], order)], torch.optim.SGD(model.parameters(), 0.0), torch.nn.CrossEntropyLoss())
+        return [e.front.table.grad for e in encs]
+
+    for order in ([0, 1], [1], [0]):
+        apart, tied = twin(False, order), twin(True, order)
+        want = sum(g.double() for g in apart if g is not None)
+        assert tied[0] is tied[1] and torch.all((tied[0].double() - want).abs() <= 2.0 ** -24 * want.abs())
+
+
+@gpu
 def test_ids_from_the_packages_datasets():
     """PartitionDataset, a stock DataLoader and DeviceResidentLoader hand ids over as float32: the same training as from whole numbers; a NaN
     skips the encoder."""
@@ -228,6 +249,25 @@ def test_refusals():
                  lambda: model.test([(data, y)], torch.nn.CrossEntropyLoss()), lambda: model.predict(data), lambda: model.get_states([(data, y)])):
         with pytest.raises(mm.UnsupportedModelError):
             call()
+
+
+def test_fronts_with_the_chains_parameters_are_refused():
+    def attempts(model):
+        data, y = batch()
+        for call in (lambda: model.train_epoch([(data, y)], torch.optim.SGD(model.parameters(), 0.1), torch.nn.CrossEntropyLoss()),
+                     lambda: model.test([(data, y)], torch.nn.CrossEntropyLoss()), lambda: model.predict(data)):
+            with pytest.raises(mm.UnsupportedModelError):
+                call()
+
+    model = build("cpu")
+    model.encoders[0].front.conv_bias = model.encoders[0].front.skip = model.encoders[0].layers[0].bias
+    attempts(model)
+    model = build("cpu")
+    model.encoders[0].front.skip = model.decoders[0].fc.bias
+    attempts(model)
+    model = build("cpu")
+    model.encoders[2].front.half()
+    attempts(model)
 
 
 def test_state_dict_and_arch(capsys):
