@@ -153,10 +153,12 @@ int mmn_seq_embed_grad(const void* ids, int ids64, const void* grad, void* out, 
     const int64_t zero_wg = small ? 0 : ceil_div(vocab, 16) < 2048 ? ceil_div(vocab, 16) : 2048;
     if (sumwg + zero_wg > MAX_GRID || ceil_div(width, 64) > 65535) return MMN_ERR_UNSUPPORTED;
     const dim3 sg((unsigned)(sumwg + zero_wg));
+    const bool join4 = width % 4 == 0 && aligned(out, 4 * size);      // (part begins on 256 bytes)
 #define SUM(T, V)                                                                                                                \
     do {                                                                                                                         \
         SEQ_LAUNCH((k_embed_sum<T, V>), sg, dim3(256), 0, st, keys[at], pos[at], (const T*)grad, (T*)out, part, present, rows, (int)vocab, width, p.chunk, nchunk, ctiles, sumwg, scale); \
-        if (nchunk > 1) SEQ_LAUNCH(k_embed_join<T>, dim3((unsigned)ceil_div(nchunk, JOIN_WAVES), (unsigned)ceil_div(width, 64)), dim3(64 * JOIN_WAVES), 0, st, keys[at], part, (T*)out, rows, (int)vocab, width, p.chunk, nchunk, scale); \
+        if (nchunk > 1 && join4) SEQ_LAUNCH((k_embed_join<T, 4>), dim3((unsigned)ceil_div(nchunk, JOIN_WAVES), (unsigned)ceil_div(width, 256)), dim3(64 * JOIN_WAVES), 0, st, keys[at], part, (T*)out, rows, (int)vocab, width, p.chunk, nchunk, scale); \
+        else if (nchunk > 1) SEQ_LAUNCH((k_embed_join<T, 1>), dim3((unsigned)ceil_div(nchunk, JOIN_WAVES), (unsigned)ceil_div(width, 64)), dim3(64 * JOIN_WAVES), 0, st, keys[at], part, (T*)out, rows, (int)vocab, width, p.chunk, nchunk, scale); \
     } while (0)
     if (type == MMN_SEQ_F32) { if (v == 4) SUM(float, 4); else SUM(float, 1); }
     else if (type == MMN_SEQ_BF16) { if (v == 8) SUM(bf16, 8); else if (v == 2) SUM(bf16, 2); else SUM(bf16, 1); }
