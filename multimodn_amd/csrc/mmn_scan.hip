@@ -20,7 +20,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 struct ScanPlan {
-    int waves, cblocks, seg, nseg, nmark, slots;
+    int waves, cblocks, seg, nseg, nmark, ck_log2, near, slots;
     int64_t grid;
     bool sorted, order;     // rows' order is made and kept with the marks; it is used
     size_t off_order, off_segh, off_segdt, off_part, off_mid, off_bc, bytes;
@@ -42,16 +42,23 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     // channels, fp32: 600 rows 790 us in segments and 965 in one piece; 1000 rows 1071 and 1045; 1500 rows 1631 and 1511).
     const int64_t waves = s->batch * s->groups * tiles;
     const int64_t want = waves >= 896 ? 1 : ceil_div(1024 * (s->lengths ? 3 : 2), waves > 0 ? waves : 1);
-    int64_t n = ceil_div(s->steps, SCAN_SEG);
+    // Marks, and so segments, every 8 steps where 16 leave half the SIMDs without a wave (64 channels, 16 states, fp32, forward and
+    // backward: 16 rows of 100 steps 44 us instead of 54, 1 row of 1024 48 instead of 60, but 256 rows of 60 72 instead of 63; 1 row of
+    // 4096 steps 72 instead of 71, for its link).
+    p.ck_log2 = s->steps <= 2048 && waves * ceil_div(s->steps, SCAN_CK) <= 512 ? 3 : 4;
+    const int ck = 1 << p.ck_log2;
+    int64_t n = ceil_div(s->steps, ck);
     n = want < n ? want : n;
     // ... and as many as it takes for a segment of the widest strided tensor to stay below 2^30 bytes (32-bit offsets in the kernels)
     int64_t stride = s->width;
     for (const int64_t t : {s->x_step, s->dt_step, s->z ? s->z_step : 0, backward ? s->dy_step : 0}) stride = t > stride ? t : stride;
-    const int64_t fits = ((int64_t)1 << 30) / (stride * 4) / SCAN_SEG * SCAN_SEG;
+    const int64_t fits = ((int64_t)1 << 30) / (stride * 4) / ck * ck;
     if (fits > 0 && ceil_div(s->steps, fits) > n) n = ceil_div(s->steps, fits);
-    p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), SCAN_SEG) * SCAN_SEG) : (s->steps > 0 ? s->steps : 1);
+    p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), ck) * ck) : (s->steps > 0 ? s->steps : 1);
     p.nseg = s->steps > 0 ? (int)ceil_div(s->steps, p.seg) : 1;
-    p.nmark = (int)ceil_div(s->steps, SCAN_CK);
+    // segments join their states themselves (64 rows of 250 steps in 16 segments: 29 us forward, by k_scan_link 26)
+    p.near = p.nseg <= (p.ck_log2 == 3 ? 16 : 8);
+    p.nmark = (int)ceil_div(s->steps, ck);
     // Backward: rows at a time, the others in turn behind them (8192 waves: eight for each SIMD)
     const int64_t most = 8192 / ((int64_t)s->groups * tiles);
     p.slots = (int)(backward && p.nseg == 1 && s->batch > most ? (most > 0 ? most : 1) : s->batch);
@@ -81,7 +88,7 @@ static bool scan_sizes_ok(const mmn_seq_scan_desc* s) {
     return s && s->batch >= 0 && s->batch <= MAX_GRID && s->steps >= 0 && s->steps <= (1 << 30) && s->width >= 1 && s->groups >= 1 && s->width % s->groups == 0 &&
            s->states >= 1 && s->states <= MMN_SEQ_MAX_STATES && s->type >= 0 && s->type <= 2;
 }
-// A segment of at least SCAN_SEG steps is addressed with 32-bit offsets; steps that share memory would not read as 0 behind the end
+// A segment of at least SCAN_CK_FEW steps is addressed with 32-bit offsets; steps that share memory would not read as 0 behind the end
 static bool scan_strides_ok(const mmn_seq_scan_desc* s, bool backward) {
     const int64_t most = 1 << 23;
     auto ok = [&](int64_t stride) { return (stride >= s->width || s->steps == 1) && stride >= 0 && stride <= most; };
@@ -104,7 +111,7 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
     a.xb = s->x_row; a.xt = s->x_step; a.dtb = s->dt_row; a.dtt = s->dt_step; a.bb = s->b_row; a.bt = s->b_step; a.bg = s->b_group;
     a.cb = s->c_row; a.ct = s->c_step; a.cg = s->c_group; a.zb = s->z_row; a.zt = s->z_step; a.dyb = s->dy_row; a.dyt = s->dy_step;
     a.steps = s->steps; a.width = s->width; a.groups = s->groups; a.states = s->states; a.softplus = s->softplus;
-    a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.cblocks = p.cblocks; a.slots = p.slots;
+    a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.ck_log2 = p.ck_log2; a.near = p.near; a.cblocks = p.cblocks; a.slots = p.slots;
     return a;
 }
 
@@ -118,7 +125,7 @@ static int scan_forward(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, false>), grid, block, 0, st, a);
         const int64_t lanes = a.batch * a.states * a.width;
-        if (p.nseg <= LINK_NEAR) {}                          // (the segments themselves: link_near)
+        if (p.near) {}                                       // (the segments themselves: link_near)
         else if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<false, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
         else SEQ_LAUNCH((k_scan_link<false, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }
@@ -133,7 +140,7 @@ static int scan_backward(const ScanArgs& a, const ScanPlan& p, float* mid, float
     if (p.nseg > 1) {
         SEQ_LAUNCH((k_scan_part<T, NP, true>), grid, block, 0, st, a);
         const int64_t lanes = a.batch * a.states * a.width;
-        if (p.nseg <= LINK_NEAR) {}                          // (the segments themselves: link_near)
+        if (p.near) {}                                       // (the segments themselves: link_near)
         else if (p.nseg > LINK_U) SEQ_LAUNCH((k_scan_link<true, 4>), dim3((unsigned)ceil_div(lanes, 64)), dim3(256), 0, st, a);
         else SEQ_LAUNCH((k_scan_link<true, 1>), dim3((unsigned)ceil_div(lanes, 256)), dim3(256), 0, st, a);
     }

@@ -175,6 +175,8 @@ SCAN = [  # batch, steps, width, groups, states, lengths, state, z, d, dt_bias, 
     (2, 40, 66, 1, 32, None, True, False, True, False, True), (1, 200, 300, 1, 4, [150], False, True, True, True, False),
     (40, 9, 65, 1, 16, None, True, True, True, True, True), (1100, 3, 70, 1, 5, "ragged", True, True, True, True, True),
     (2100, 2, 36, 6, 8, None, False, True, True, True, True), (2, 48, 560, 1, 5, [-3, 1000], False, True, True, True, True),
+    (90, 100, 64, 1, 16, "ragged", True, True, True, True, True), (60, 250, 40, 2, 6, None, True, False, True, True, True),
+    (1, 2049, 30, 1, 4, None, True, True, True, True, True), (3, 1100, 20, 1, 3, [1100, 1, 555], False, True, True, True, True),
 ]
 
 
