@@ -16,7 +16,6 @@ HEADERS = ("mmn_hip.h", "mmn_sequence.h")
 UNITS = ("mmn_kernels.hip", "mmn_sequence.hip", "mmn_scan.hip")
 #: packed 32-bit float operations off: some of their forms have given wrong results on this hardware
 _NO_PACKED = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
-UNIT_FLAGS = {unit: _NO_PACKED for unit in ("mmn_sequence.hip", "mmn_scan.hip")}
 
 
 def hipcc_path() -> str:
@@ -88,12 +87,12 @@ def build(force: bool = False, verbose: bool = False, only=None) -> str:
     # -amdgpu-mfma-vgpr-form: accumulators stay in VGPRs (gfx950's register file is unified).  With AGPR accumulators
     # hipcc rotated k_wgrad's sixteen accumulator tiles through v_accvgpr_read / _write pairs in every unrolled loop
     # body (reads that wait for the MFMA that produced the tile): k_wgrad 18.1 -> 17.5 us, the step -1.4 us.
-    flags = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-mfma-vgpr-form", f"-I{INC}"]
+    flags = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-mfma-vgpr-form", *_NO_PACKED, f"-I{INC}"]
     os.makedirs(OBJ, exist_ok=True)
     objects, running = [], []
     for unit in UNITS:
         obj = os.path.join(OBJ, unit.replace(".hip", ".o"))
-        cmd = [hipcc_path(), *flags, *UNIT_FLAGS.get(unit, ()), "-c", os.path.join(CSRC, unit), "-o", obj]
+        cmd = [hipcc_path(), *flags, "-c", os.path.join(CSRC, unit), "-o", obj]
         if unit == "mmn_sequence.hip":                     # (the unit that says what the library was built from: a quick one)
             cmd.insert(1, f'-DMMN_SOURCE_HASH="{source_hash()}"')
         objects.append(obj)
