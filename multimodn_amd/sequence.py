@@ -148,7 +148,7 @@ class ScanGrads(NamedTuple):
 
 
 class ScanSaved(NamedTuple):
-    """What selective_scan_grad needs of a forward pass: its inputs, and the states at every 16th step."""
+    """What selective_scan_grad needs of a forward pass: its inputs, and the states at every 16th step (8th, for small problems)."""
     x: Tensor
     dt: Tensor
     a: Tensor
