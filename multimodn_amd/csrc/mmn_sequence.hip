@@ -186,7 +186,7 @@ static int conv_vec(const mmn_seq_conv_desc* c) {
         for (const void* q : ptr) if (!aligned(q, (size_t)v * size)) return false;
         return c->width % v == 0 && c->x_row % v == 0 && c->x_step % v == 0 && c->dy_row % v == 0 && c->dy_step % v == 0;
     };
-    return fits(4) ? 4 : 1;                              // (8 of 16 bits: 23 us instead of 20 for 8 x 2048 x 1024, fewer waves)
+    return fits(4) ? 4 : 1;                              // (8 of 16 bits: 22.5 us instead of 18 for 8 x 2048 x 1024 ragged, fewer waves)
 }
 #define CONV_TAPS(KERN, T, V, ...)                                                   \
     do {                                                                             \
