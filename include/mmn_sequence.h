@@ -51,7 +51,8 @@ int mmn_seq_conv_step(const mmn_seq_conv_desc* c, void* stream);
 
 /* dt = softplus(dt_raw + dt_bias); h = exp(dt a) h + dt x b; y = (sum_n c h + d x) * silu(z).  a [width][states], b and c
  * [batch][steps][groups][states] (states adjacent), the rest [batch][steps][width] (channels adjacent) with the given strides; y, dx,
- * ddt, dz, db, dc, states [batch][width][states] dense.  d, dt_bias, z, lengths, state, state_out may be NULL. */
+ * ddt, dz, db, dc, states [batch][width][states] dense.  The step strides of x, dt, z, dy are from width to 2^23, those of one step or
+ * none are not used.  d, dt_bias, z, lengths, state, state_out may be NULL. */
 typedef struct mmn_seq_scan_desc {
     const void *x, *dt, *b, *c, *z;
     const float *a, *d, *dt_bias, *state;

@@ -17,6 +17,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 #include "seq_host.inc"
 
+// Steps' distance in x, dt, z or dy.  Of one step, or none, it is the width, whatever the caller says: the kernels walk steps in pieces
+// and rely on those behind the last lying behind the buffer's end.
+static int64_t step_of(const mmn_seq_scan_desc* s, int64_t stride) { return s->steps > 1 ? stride : s->width; }
+
 static int padded_states(int n) { return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 struct ScanPlan {
@@ -51,7 +55,8 @@ static ScanPlan scan_plan(const mmn_seq_scan_desc* s, bool backward) {
     n = want < n ? want : n;
     // ... and as many as it takes for a segment of the widest strided tensor to stay below 2^30 bytes (32-bit offsets in the kernels)
     int64_t stride = s->width;
-    for (const int64_t t : {s->x_step, s->dt_step, s->z ? s->z_step : 0, backward ? s->dy_step : 0}) stride = t > stride ? t : stride;
+    for (const int64_t t : {s->x_step, s->dt_step, s->z ? s->z_step : 0, backward ? s->dy_step : 0})
+        if (step_of(s, t) > stride) stride = step_of(s, t);
     const int64_t fits = ((int64_t)1 << 30) / (stride * 4) / ck * ck;
     if (fits > 0 && ceil_div(s->steps, fits) > n) n = ceil_div(s->steps, fits);
     p.seg = n > 1 ? (int)(ceil_div(ceil_div(s->steps, n), ck) * ck) : (s->steps > 0 ? s->steps : 1);
@@ -91,7 +96,7 @@ static bool scan_sizes_ok(const mmn_seq_scan_desc* s) {
 // A segment of at least SCAN_CK_FEW steps is addressed with 32-bit offsets; steps that share memory would not read as 0 behind the end
 static bool scan_strides_ok(const mmn_seq_scan_desc* s, bool backward) {
     const int64_t most = 1 << 23;
-    auto ok = [&](int64_t stride) { return (stride >= s->width || s->steps == 1) && stride >= 0 && stride <= most; };
+    auto ok = [&](int64_t stride) { return step_of(s, stride) >= s->width && step_of(s, stride) <= most; };
     return s->width <= most && ok(s->x_step) && ok(s->dt_step) && (!s->z || ok(s->z_step)) && (!backward || ok(s->dy_step));
 }
 
@@ -108,8 +113,8 @@ static ScanArgs scan_args(const mmn_seq_scan_desc* s, const ScanPlan& p, char* w
     a.seg_h = (float*)(ws + p.off_segh); a.seg_dt = (float*)(ws + p.off_segdt); a.marks = s->marks;
     a.part = (float*)(ws + p.off_part); a.bc_part = (float*)(ws + p.off_bc);
     a.batch = s->batch;
-    a.xb = s->x_row; a.xt = s->x_step; a.dtb = s->dt_row; a.dtt = s->dt_step; a.bb = s->b_row; a.bt = s->b_step; a.bg = s->b_group;
-    a.cb = s->c_row; a.ct = s->c_step; a.cg = s->c_group; a.zb = s->z_row; a.zt = s->z_step; a.dyb = s->dy_row; a.dyt = s->dy_step;
+    a.xb = s->x_row; a.xt = step_of(s, s->x_step); a.dtb = s->dt_row; a.dtt = step_of(s, s->dt_step); a.bb = s->b_row; a.bt = s->b_step; a.bg = s->b_group;
+    a.cb = s->c_row; a.ct = s->c_step; a.cg = s->c_group; a.zb = s->z_row; a.zt = step_of(s, s->z_step); a.dyb = s->dy_row; a.dyt = step_of(s, s->dy_step);
     a.steps = s->steps; a.width = s->width; a.groups = s->groups; a.states = s->states; a.softplus = s->softplus;
     a.seg = p.seg; a.nseg = p.nseg; a.nmark = p.nmark; a.ck_log2 = p.ck_log2; a.near = p.near; a.cblocks = p.cblocks; a.slots = p.slots;
     return a;

@@ -1,0 +1,80 @@
+"""Calls of the sequence operators that their documentation allows and that once answered wrongly or were refused."""
+import pytest
+import torch
+
+import sequence_oracle as O
+from multimodn_amd import sequence as seq
+from test_sequence import normal, rng
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("gated", [True, False])
+def test_one_step_of_channels_in_front(dtype, gated):
+    """[batch, width, 1] turned to [batch, 1, width]: a step's stride is 1, which no other step uses.  As the dense copies, every gradient."""
+    g = rng(40)
+    B, W, N = 5, 70, 6
+    turned = lambda: normal(g, B, W, 1, dtype=dtype).transpose(1, 2)
+    x, dt, dy = turned(), turned(), turned()
+    z = turned() if gated else None
+    assert x.stride() == (W, 1, 1)
+    a, d, bias = -torch.rand(W, N, generator=g).cuda() - 0.1, normal(g, W), normal(g, W)
+    b, c, s, ds = normal(g, B, 1, N, dtype=dtype), normal(g, B, 1, N, dtype=dtype), normal(g, B, W, N), normal(g, B, W, N)
+    copy = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device="cuda").copy_(t)
+
+    def both(x, dt, z, dy):
+        y, out, saved = seq.selective_scan_forward(x, dt, a, b, c, d, z, bias, state=s, return_state=True)
+        return (y, out) + tuple(seq.selective_scan_grad(dy, saved, ds))
+
+    dense = [copy(t) for t in (x, dt, z, dy)]
+    assert dense[0].stride() == (W, W, 1)
+    want = O.scan(x, dt, a, b.unsqueeze(2), c.unsqueeze(2), d, z, bias, True, None, s, dy, ds)
+    for got in (both(*dense), both(x, dt, z, dy), both(dense[0], dense[1], dense[2], dy), both(x, dt, z, dense[3])):
+        for p, q in zip(got, both(*dense)):
+            assert (p is None and q is None) or torch.equal(p, q)
+        # d(d) is B products of dy, the gate and x: two roundings each in the gate, one in each product and sum
+        O.check(got[7], *want["d"], B + 8, "dd")
+    conv = normal(g, W, 4)
+    for p, q in zip(seq.causal_conv_grad(dy, x, conv, bias), seq.causal_conv_grad(dense[3], dense[0], conv, bias)):
+        assert (p is None and q is None) or torch.equal(p, q)
+    leaf = dense[0].clone().requires_grad_(True)                              # a gradient that autograd itself hands over in this layout
+    skip = d.clone().requires_grad_(True)
+    y = seq.selective_scan(leaf, dense[1], a, b, c, skip, dense[2], bias)
+    (grad,) = torch.autograd.grad(y.transpose(1, 2), skip, dy.transpose(1, 2))
+    y, _, saved = seq.selective_scan_forward(dense[0], dense[1], a, b, c, d, dense[2], bias)
+    assert torch.equal(grad, seq.selective_scan_grad(dense[3], saved).d)
+
+
+@gpu
+def test_one_step_does_not_read_other_channels():
+    """An infinity in one channel stays there."""
+    g = rng(41)
+    x = normal(g, 2, 9, 1)
+    x[:, 4] = float("inf")
+    x = x.transpose(1, 2)
+    dt, b = normal(g, 2, 1, 9), normal(g, 2, 1, 3)
+    y, state = seq.selective_scan(x, dt, -torch.ones(9, 3, device="cuda"), b, b, return_state=True)
+    others = [0, 1, 2, 3, 5, 6, 7, 8]
+    assert torch.isfinite(y[..., others]).all() and torch.isfinite(state[:, others]).all()
+
+
+@gpu
+def test_one_step_or_none_with_any_stride():
+    """The stride of a dimension of one step, or of none, is never used: one step of a large time-major batch, no steps of channels in front."""
+    g = rng(42)
+    B, W = 66000, 128                                                         # B * W > 2^23
+    x, dt = normal(g, 1, B, W).transpose(0, 1), normal(g, 1, B, W).transpose(0, 1)
+    b = normal(g, B, 1, 2)
+    a = -torch.ones(W, 2, device="cuda")
+    assert x.stride(1) > 1 << 23
+    y, _, saved = seq.selective_scan_forward(x, dt, a, b, b)
+    dense = [torch.empty(B, 1, W, device="cuda").copy_(t) for t in (x, dt)]
+    y2, _, saved2 = seq.selective_scan_forward(*dense, a, b, b)
+    assert torch.equal(y, y2)
+    assert all(torch.equal(p, q) for p, q in zip(seq.selective_scan_grad(x, saved), seq.selective_scan_grad(dense[0], saved2)) if p is not None)
+    none = torch.zeros(4, W, 0, device="cuda").transpose(1, 2)
+    s = normal(g, 4, W, 2)
+    y, out = seq.selective_scan(none, none, a, b[:4, :0], b[:4, :0], state=s, return_state=True)
+    assert y.shape == (4, 0, W) and torch.equal(out, s)
