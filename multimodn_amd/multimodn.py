@@ -572,11 +572,10 @@ class MultiModN(nn.Module):
             found = self._slot_features(data, self.get_encoder_iterable(encoder_sequence, False, train=False))
         return [found[k] if k in found else t.to(self.device) for k, t in enumerate(data)]
 
-    def _front_grads(self) -> None:
-        """Every front parameter's .grad at its own, zeroed place of one buffer: the backward adds into it, and an optimizer sees the same
-        addresses in every step."""
-        params = list({id(p): p for enc in self.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters()
-                       if p.requires_grad}.values())
+    def _front_grads(self):
+        """Every front parameter's .grad at its own, zeroed place of one buffer (None where it is frozen): the backward adds into it, and an
+        optimizer sees the same addresses in every step.  Returns (all front parameters, their places)."""
+        params = list({id(p): p for enc in self.encoders if isinstance(enc, SequenceEncoder) for p in enc.front.parameters()}.values())
         buf = self.__dict__.get("_front_grad_buf")
         sig = tuple((id(p), tuple(p.shape), p.device) for p in params)
         if buf is None or buf[0] != sig:
@@ -589,7 +588,8 @@ class MultiModN(nn.Module):
             buf = self.__dict__["_front_grad_buf"] = (sig, flat, views)
         buf[1].zero_()
         for p, g in zip(params, buf[2]):
-            p.grad = g
+            p.grad = g if p.requires_grad else None
+        return params, buf[2]
 
     def _train_steps_sequences(self, train_loader, optimizer, log_interval=None, logger=None):
         """The batch loop of train_epoch for models with a SequenceEncoder: the features are made with the step's own parameters, the
@@ -618,7 +618,10 @@ class MultiModN(nn.Module):
             masks = eng.draw_dropout_masks(b, self.dropout_mask_provider) if eng.dropout_encoders else None
             eng.local_step(b, alpha, beta, accumulate=True)
             self.__dict__["train_steps_launched"] = self.__dict__.get("train_steps_launched", 0) + 1
-            self._front_grads()
+            places = self._front_grads()
+            if hasattr(optimizer, "expect_gradients"):
+                optimizer.expect_gradients(*places)
+                optimizer.expect_gradients(eng.params, eng.grad_views)
             ran = {k for k, _ in exec_pairs}
             for k, e in pairs:
                 if k in features and k in ran and features[k].requires_grad:

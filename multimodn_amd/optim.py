@@ -188,6 +188,15 @@ class Adam(Optimizer):
             r.skip_host = tuple([0] * len(r.params))
         return self.descriptor(r, group)
 
+    def expect_gradients(self, params, places) -> None:
+        """Where these parameters' gradients will be.  The first step() lays out every parameter of a group together with its
+        gradient, also those whose gradient is None in that step (an encoder without data, a frozen parameter): MultiModN names
+        the places of models whose step is not fused."""
+        if not hasattr(self, "_last_grads"):
+            self._last_grads = {}
+        for p, g in zip(params, places):
+            self._last_grads[id(p)] = g
+
     def mark_fused_step(self) -> None:
         self._fused_pending = True
 
