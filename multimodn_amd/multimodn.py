@@ -647,6 +647,8 @@ class MultiModN(nn.Module):
     def _run_step(self, eng, data, target, encoder_sequence, train: bool, batch_global: Optional[int] = None,
                   optimizer=None):
         """One step on its own (no look-ahead): what test() / the parity tests / smoke() drive."""
+        if train and self._has_sequences():
+            raise UnsupportedModelError("a single training step has no gradient for a SequenceEncoder's front: train_epoch trains it")
         data = self._with_features(data, encoder_sequence)
         mode = self._nan_mode(eng, optimizer, train)
         st = self._make_step(data, target, encoder_sequence, mode, train)

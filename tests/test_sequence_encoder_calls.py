@@ -61,3 +61,13 @@ def test_adam_whose_first_batch_is_incomplete(kind):
         else:
             assert p.grad is not None and float(opts[0].state[p]["step"]) == (1 if still else 2)
             assert not p.grad.any() or not torch.equal(p, later[n]), n
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_single_training_step_is_refused(device):
+    """It would train the chain alone (the features are made without a graph)."""
+    model = build(device)
+    data, y = batch()
+    eng = model._get_engine(ROWS) if device == "cuda" else None
+    with pytest.raises(mm.UnsupportedModelError, match="train_epoch"):
+        model._run_step(eng, data, y, None, True)
