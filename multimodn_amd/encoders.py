@@ -128,8 +128,9 @@ class SequenceFeatures(nn.Module):
 
     A row ends behind its last id >= 0: pad with -1.  An id outside the vocabulary inside a row is a step without a token (its
     embedding is 0).  A row without any token has the features 0.  The datasets of this package hand every slot over as float32: the
-    whole numbers there are the ids, and a row with a NaN has NaN features, so that its batch skips the encoder like any
-    other modality's (multimodn/multimodn.py:168)."""
+    whole numbers there are the ids, and a row with anything else - a NaN, an infinity, a fraction - has NaN features, so that
+    its batch skips the encoder like any other modality's (multimodn/multimodn.py:168).  A floating type that does not hold every id
+    of the vocabulary is refused (float16 holds whole numbers to 2048, bfloat16 to 256, float32 to 2^24)."""
 
     def __init__(self, vocabulary: int, width: int, states: int = 16, taps: int = 4, rank: Optional[int] = None,
                  device: Optional[torch.device] = None):
@@ -158,8 +159,11 @@ class SequenceFeatures(nn.Module):
             raise ValueError(f"token ids must be a [batch, steps] tensor of whole numbers, not {list(ids.shape)} of {ids.dtype}")
         missing = None
         if ids.is_floating_point():
-            missing = torch.isnan(ids).any(1, keepdim=True)
-            ids = torch.where(torch.isfinite(ids), ids, -1.0).long()
+            if self.vocabulary > 2 / torch.finfo(ids.dtype).eps:
+                raise ValueError(f"{ids.dtype} does not hold all {self.vocabulary} token ids: pass them as whole numbers")
+            whole = torch.isfinite(ids) & (ids == ids.trunc())
+            missing = ~whole.all(1, keepdim=True)
+            ids = torch.where(whole, ids, -1.0).clamp(-1, self.vocabulary).long()      # (a whole number of any size, which int64 may not hold)
         elif ids.dtype not in (torch.int32, torch.int64):
             ids = ids.long()
         steps = torch.arange(1, ids.shape[1] + 1, device=ids.device)

@@ -71,3 +71,34 @@ def test_a_single_training_step_is_refused(device):
     eng = model._get_engine(ROWS) if device == "cuda" else None
     with pytest.raises(mm.UnsupportedModelError, match="train_epoch"):
         model._run_step(eng, data, y, None, True)
+
+
+@gpu
+def test_floating_ids_that_are_not_whole_numbers():
+    """Rows with a fraction or an infinity have NaN features, the others those of the same ids as whole numbers."""
+    front = build(seed=9).encoders[0].front
+    ids = torch.tensor([[1.0, 2.0, 3.0], [1.0, 3.7, 2.0], [1.0, float("inf"), 2.0], [-0.5, 1.0, 2.0], [4.0, -1.0, V], [float("nan"), 1.0, 2.0],
+                        [2.0, -float("inf"), -1.0], [-1.0, -1.0, -1.0]]).cuda()
+    for kind in (torch.float32, torch.float64, torch.float16, torch.bfloat16):
+        got = front(ids.to(kind))
+        good = [0, 4, 7]
+        assert torch.equal(got[good], front(ids[good].long()))
+        assert torch.isnan(got[[1, 2, 3, 5, 6]]).all()
+    far = torch.tensor([[1.0, 2.0, 1e30], [-1e30, 2.0, 3.0]]).cuda()              # outside the vocabulary; a step without a token
+    assert torch.equal(front(far), front(torch.tensor([[1, 2, V], [-1, 2, 3]]).cuda()))
+    data, y = batch(5)
+    data[0] = data[0].float()
+    data[0][3, 2] = 1.5
+    model = build(seed=4)
+    model.train_epoch([(data, y)], torch.optim.SGD(model.parameters(), 1e-2), torch.nn.CrossEntropyLoss())
+    assert all(p.grad is None for p in model.encoders[0].parameters())
+    assert all(torch.isfinite(p.grad).all() for e in (1, 2) for p in model.encoders[e].parameters())
+
+
+def test_floating_types_that_do_not_hold_the_vocabulary_are_refused():
+    for vocabulary, kind in ((257, torch.bfloat16), (2049, torch.float16), ((1 << 24) + 1, torch.float32)):
+        front = mm.SequenceFeatures(vocabulary, 1, states=1, taps=2)
+        with pytest.raises(ValueError, match="token ids"):
+            front(torch.zeros(2, 3, dtype=kind))
+        with pytest.raises(mm.hip.MmnError):                                  # (ids of a type that holds them go on to the operators)
+            front(torch.zeros(2, 3, dtype=torch.float64))
