@@ -133,7 +133,8 @@ def load(path: Optional[str] = None) -> C.CDLL:
             f"__graft_entry__ as g; g.build()'` (needs hipcc). There is no CPU fallback for the "
             f"training hot path.")
     lib = C.CDLL(p)
-    missing = [s for s in ABI_SYMBOLS + SEQUENCE_SYMBOLS if not hasattr(lib, s)]
+    # (a library of the training path alone, mmn_kernels.hip by itself, has no sequence operators: load_binding refuses it)
+    missing = [s for s in ABI_SYMBOLS + (SEQUENCE_SYMBOLS if p == LIB_PATH else ()) if not hasattr(lib, s)]
     if missing:
         raise MmnError(f"{p} does not export {missing}")
     vp, i32, f32 = C.c_void_p, C.c_int, C.c_float
@@ -257,7 +258,8 @@ def load(path: Optional[str] = None) -> C.CDLL:
             ("mmn_seq_conv_step", i32, [conv, vp]), ("mmn_seq_scan_marks", size, [scan]), ("mmn_seq_scan_bytes", size, [scan, i32]),
             ("mmn_seq_scan", i32, [scan, vp, size, vp]), ("mmn_seq_scan_grad", i32, [scan, vp, size, vp]), ("mmn_seq_scan_step", i32, [scan, vp]),
             ("mmn_seq_input_grad", i32, [vp, vp, vp, i64, i32, i32, vp])):
-        getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
+        if hasattr(lib, name):
+            getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
     if lib.mmn_version() != VERSION:
         raise MmnError(f"{p}: ABI version {lib.mmn_version()} != expected {VERSION}; rebuild")
     lib.mmn_source_hash.restype = C.c_char_p
@@ -289,8 +291,11 @@ def load_binding():
     global _binding
     if _binding is not None:
         return _binding
-    load()
+    lib = load()
     path = os.environ.get("MMN_LIB_PATH") or LIB_PATH
+    missing = [s for s in SEQUENCE_SYMBOLS if not hasattr(lib, s)]
+    if missing:
+        raise MmnError(f"{path} has no sequence operators (it does not export {missing})")
     try:
         from . import _binding as m
     except ImportError as e:
