@@ -59,15 +59,6 @@ def _rank(item) -> int:
     return _RANK_REST
 
 
-# The check that the electric fence is live takes a GPU memory fault on purpose.  On shared machines such a fault ends more than the child
-# process that takes it (the driver may reset the card under everybody's work): it runs only where that is asked for.
-_FAULTS_ON_PURPOSE = ("test_the_fence_is_live",)
-
-
 def pytest_collection_modifyitems(session, config, items):
-    if os.environ.get("MMN_EFENCE_LIVE", "0") in ("", "0"):
-        for it in items:
-            if it.name in _FAULTS_ON_PURPOSE:
-                it.add_marker(pytest.mark.skip(reason="makes the GPU fault on purpose; MMN_EFENCE_LIVE=1 on a machine of your own runs it"))
     order = {id(it): k for k, it in enumerate(items)}
     items.sort(key=lambda it: (_rank(it), order[id(it)]))

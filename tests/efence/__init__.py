@@ -4,7 +4,7 @@
 becomes its own mapping that ends flush against unmapped address space, so that a kernel reading or writing past the
 end of any tensor faults deterministically.  Must run before the process makes its first device allocation.
 `MMN_EFENCE=1 python -m pytest tests -m gpu` runs the whole suite that way (tests/conftest.py); tools/fault_hunt.py
-runs the generic tier's random sweeps seed by seed in child processes under it."""
+runs the generic tier's random sweeps under it."""
 import os
 import subprocess
 
