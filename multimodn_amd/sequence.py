@@ -192,7 +192,10 @@ def selective_scan(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, d: Op
 
     x, dt, z [batch, steps, width]; a [width, states] with 1 to 32 states; b, c [batch, steps, states], or [batch, steps, groups,
     states] where each group serves width / groups neighbouring channels; d, dt_bias [width].  `state` [batch, width, states] is h in
-    front of the first step (None: zeros); with `return_state` the result is (y, h behind each row's last step)."""
+    front of the first step (None: zeros); with `return_state` the result is (y, h behind each row's last step).
+
+    States may grow (dt' a > 0).  Long sequences are walked in segments, whose factors exp(a sum of dt') are 32 bits too: where one
+    overflows, so does every state that is not 0 at its beginning."""
     if _any_grad(x, dt, a, b, c, d, z, dt_bias, state):
         y, out = _Scan.apply(x, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, return_state)
     else:

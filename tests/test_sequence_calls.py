@@ -78,3 +78,30 @@ def test_one_step_or_none_with_any_stride():
     s = normal(g, 4, W, 2)
     y, out = seq.selective_scan(none, none, a, b[:4, :0], b[:4, :0], state=s, return_state=True)
     assert y.shape == (4, 0, W) and torch.equal(out, s)
+
+
+@gpu
+@pytest.mark.parametrize("growth", [0.5, 4.0])
+@pytest.mark.parametrize("rows,steps,states", [(1, 2000, 3), (1, 4096, 16), (300, 300, 3), (40, 250, 5), (2, 100, 30)])
+def test_states_that_grow_from_zero(rows, steps, states, growth):
+    """a > 0: while nothing has come in a state stays 0, in however many segments the steps are walked; the same backwards behind the last
+    gradient.  All rows are alike: the statement is made for one."""
+    g = rng(43)
+    D = 6
+    x, dy, dt = torch.zeros(1, steps, D), torch.zeros(1, steps, D), torch.ones(1, steps, D)
+    x[:, -3:], dy[:, :3] = torch.randn(1, 3, D, generator=g), torch.randn(1, 3, D, generator=g)
+    b, c = torch.randn(1, steps, states, generator=g), torch.randn(1, steps, states, generator=g)
+    a = torch.full((D, states), growth)
+    want = O.scan(x, dt, a, b.unsqueeze(2), c.unsqueeze(2), None, None, None, False, None, None, dy)
+    case = [t.expand(rows, *t.shape[1:]).cuda() for t in (x, dt, b, c, dy)]
+    y, state, saved = seq.selective_scan_forward(case[0], case[1], a.cuda(), case[2], case[3], softplus=False, return_state=True)
+    grads = seq.selective_scan_grad(case[4], saved)
+    n = 3 * 3 + 12 + states + 24                                              # (three steps with anything in them; as scan_terms of the other tests)
+    for i in (0, rows - 1):
+        O.check(y[i:i + 1], *want["y"], n, "y")
+        O.check(state[i:i + 1], *want["state"], n, "state")
+        for name in ("x", "dt"):
+            O.check(getattr(grads, name)[i:i + 1], *want[name], 2 * n, "d" + name)
+        for name in ("b", "c"):
+            O.check(getattr(grads, name)[i:i + 1], *want[name], 2 * n + D, "d" + name)
+    assert not grads.a.any()                                                  # (every product of a gradient and a state is 0)
