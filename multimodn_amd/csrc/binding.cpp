@@ -2,7 +2,9 @@
 // outputs and workspaces from torch's allocator, the call.  Host code only; multimodn_amd/sequence.py is its one user.
 // (In Python the checks and the descriptors of a one-step pair of calls took 38 of 44 us.)
 #include <torch/extension.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <dlfcn.h>
+#include <unordered_set>
 
 #include "mmn_sequence.h"
 
@@ -129,13 +131,27 @@ Tensor state_pair(const Opt& state, const Opt& out_state) {
 void moved(const Tensor& t) {                                        // written through its address: autograd's saved copies are stale
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
-// Does an autograd graph made on the default stream still hold this leaf?  A backward pass captured on another stream would hand it
-// the gradient there, which no capture allows and ends the process.
-bool held_eagerly(const Opt& t) {
-    if (!t || !t->requires_grad() || !t->is_leaf()) return false;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : c10::nullopt;
-    return stream && stream->id() == 0;
+// Does a backward pass from one of these tensors meet a node, or a leaf's accumulator, that was made on another stream than the current
+// one?  Autograd runs each node, and adds to each leaf, on the stream on which it was made.  A captured backward pass may not go there:
+// on the default stream that ends the process.
+bool made_elsewhere(const std::vector<Opt>& tensors) {
+    const c10::impl::VirtualGuardImpl guard(at::kCUDA);
+    std::vector<torch::autograd::Node*> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    std::vector<std::shared_ptr<torch::autograd::Node>> kept;            // (an accumulator is held by the graphs that use it)
+    auto take = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+        if (node && seen.insert(node.get()).second) { kept.push_back(node); todo.push_back(node.get()); }
+    };
+    for (const Opt& t : tensors)
+        if (t && t->requires_grad()) take(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        torch::autograd::Node* const node = todo.back();
+        todo.pop_back();
+        const auto stream = node->stream();
+        if (stream && stream->device_type() == at::kCUDA && *stream != guard.getStream(stream->device())) return true;
+        for (const auto& edge : node->next_edges()) take(edge.function);
+    }
+    return false;
 }
 const void* ptr(const Opt& t) { return t ? t->data_ptr() : nullptr; }
 template <typename T> T* at_of(const Opt& t) { return t ? (T*)t->data_ptr() : nullptr; }
@@ -377,7 +393,7 @@ Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tenso
 PYBIND11_MODULE(_binding, m) {
     m.def("bind", &bind);
     m.def("source_hash", [] { return std::string(MMN_SOURCE_HASH); });
-    m.def("held_eagerly", &held_eagerly);
+    m.def("made_elsewhere", &made_elsewhere);
     m.def("embed", &embed);
     m.def("embed_grad", &embed_grad);
     m.def("conv", &conv);

@@ -12,9 +12,9 @@ table) and the scan's states are float32, and so are all sums inside.  Tensors a
 any other strides (anything else is copied); results are dense.  `lengths` ([batch], whole numbers) says how many steps of each row
 count: what stands behind them is not read, gives 0 and leaves the states as they are.  Results do not change from run to run.
 
-Everything runs on the current stream of the tensors' device, may be captured into a graph (with autograd: once no eager graph holds the
-leaves any more; refused before), and has no CPU or torch-op fallback: off
-an AMD GPU these functions raise.  The reference has no counterpart: its recurrent encoders (multimodn/encoders/rnn_encoder.py,
+Everything runs on the current stream of the tensors' device, may be captured into a graph (with autograd: once no graph made on another
+stream holds the tensors, or the leaves they come from, any more; refused before), and has no CPU or torch-op fallback: off an AMD GPU
+these functions raise.  The reference has no counterpart: its recurrent encoders (multimodn/encoders/rnn_encoder.py,
 lstm_encoder.py) are torch modules.
 """
 from __future__ import annotations
@@ -40,10 +40,10 @@ def _any_grad(*tensors: Optional[Tensor]) -> bool:
 
 
 def _check_capture(*tensors: Optional[Tensor]) -> None:
-    """Refuses to record for autograd, inside a graph capture, on a leaf that an eager graph still holds."""
-    if tensors[0].is_cuda and torch.cuda.is_current_stream_capturing() and any(_native().held_eagerly(t) for t in tensors):
-        raise hip.MmnError("an autograd graph made outside this capture still holds one of these leaves: drop its outputs and losses first "
-                           "(the captured backward pass would add to the leaf on the default stream), or call under torch.no_grad()")
+    """Refuses to record for autograd, inside a graph capture, on what a graph made outside it holds."""
+    if tensors[0].is_cuda and torch.cuda.is_current_stream_capturing() and _native().made_elsewhere(tensors):
+        raise hip.MmnError("an autograd graph made outside this capture, on another stream, holds these tensors or leaves they come from: drop its "
+                           "outputs and losses first (the captured backward pass would go on to that stream), or call under torch.no_grad()")
 
 
 # ---------------------------------------------------------------------------------------------------------------- embedding

@@ -1,9 +1,12 @@
 """Calls of the sequence operators that their documentation allows and that once answered wrongly or were refused."""
+import os
+
 import pytest
 import torch
 
 import sequence_oracle as O
-from multimodn_amd import sequence as seq
+import multimodn_amd as mm
+from multimodn_amd import hip, sequence as seq
 from test_sequence import normal, rng
 
 gpu = pytest.mark.gpu
@@ -105,3 +108,69 @@ def test_states_that_grow_from_zero(rows, steps, states, growth):
         for name in ("b", "c"):
             O.check(getattr(grads, name)[i:i + 1], *want[name], 2 * n + D, "d" + name)
     assert not grads.a.any()                                                  # (every product of a gradient and a state is 0)
+
+
+fence = pytest.mark.skipif(os.environ.get("MMN_EFENCE", "0") not in ("", "0"), reason="the electric fence's allocator fills new memory, which a capture does not allow")
+
+
+@gpu
+@fence
+@pytest.mark.parametrize("where", ["default", "side"])
+def test_captures_refuse_what_another_stream_holds(where):
+    """A leaf, or a tensor that comes from one, whose autograd graph was made outside the capture: refused before anything is recorded for
+    autograd.  Without gradients, and once those graphs are gone, the same calls are captured."""
+    g = rng(44)
+    B, L, D, N = 2, 9, 16, 4
+    source = normal(g, B, L, D).requires_grad_(True)
+    w, a = normal(g, D, 3).requires_grad_(True), (-torch.rand(D, N, generator=g).cuda()).requires_grad_(True)
+    b = normal(g, B, L, N)
+    stream = torch.cuda.Stream() if where == "side" else torch.cuda.current_stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        x = source * 2                                                        # made outside: a node and, behind it, a leaf's accumulator
+        held = (w * 1, a * 1)
+    torch.cuda.synchronize()
+    dense = normal(g, B, L, D)
+    for call in (lambda: seq.causal_conv(dense, w), lambda: seq.causal_conv(x, w.detach()), lambda: seq.selective_scan(dense, dense, a, b, b),
+                 lambda: seq.selective_scan(dense, x, a.detach(), b, b), lambda: seq.selective_scan(source * 3, dense, a.detach(), b, b),
+                 lambda: seq.causal_conv(dense, torch.exp(w))):
+        with pytest.raises(hip.MmnError, match="drop its"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        torch.cuda.synchronize()
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = seq.causal_conv(x, w)
+        graph.replay()
+        assert torch.equal(y, seq.causal_conv(x, w))
+    del held, x, graph
+    call = lambda: torch.autograd.grad(seq.causal_conv(source * 2, torch.exp(w)), (source, w), dense)
+    want = [t.clone() for t in call()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for turn in range(3):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), turn
+
+
+@gpu
+@fence
+def test_captures_of_a_front_refuse_what_another_stream_holds():
+    """SequenceFeatures with a frozen table: its projections' weights are the leaves that an eager graph holds."""
+    torch.manual_seed(45)
+    front = mm.SequenceFeatures(20, 16, states=4, device="cuda")
+    front.table.requires_grad_(False)
+    ids = torch.randint(0, 20, (3, 9), generator=rng(45)).cuda()
+    features = front(ids)
+    torch.cuda.synchronize()
+    with pytest.raises(hip.MmnError, match="drop its"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            front(ids)
+    torch.cuda.synchronize()
+    assert torch.equal(features, front(ids))
