@@ -1,9 +1,13 @@
 """Calls of models with a SequenceEncoder that their documentation allows and that once failed, answered wrongly or were not refused."""
+import copy
+
 import pytest
 import torch
 
 import multimodn_amd as mm
-from test_sequence_encoder import ROWS, S, STEPS, V, WIDTH, batch, build
+from helpers import rel_err
+from test_hip_parity import KERNEL_MODES, set_mode
+from test_sequence_encoder import ROWS, STEPS, V, batch, build, plain_step
 
 gpu = pytest.mark.gpu
 
@@ -102,3 +106,29 @@ def test_floating_types_that_do_not_hold_the_vocabulary_are_refused():
             front(torch.zeros(2, 3, dtype=kind))
         with pytest.raises(mm.hip.MmnError):                                  # (ids of a type that holds them go on to the operators)
             front(torch.zeros(2, 3, dtype=torch.float64))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [16, 257])
+@pytest.mark.parametrize("mode", list(KERNEL_MODES))
+def test_fronts_train_through_every_tier_of_the_chain(mode, rows, monkeypatch):
+    """The gradient that leaves the chain at an encoder's input, whichever kernels ran the chain: gradients of all parameters against 64 bits
+    at the framework's own sizes (state 128, hidden (32, 32), four encoders).  A sum of n products in 32 bits is off by n 2^-24 of its terms'
+    size: an encoder's layers and state update sum 64 + 128, 32 and 32 values and the same backwards, so four encoders some 2100, the front
+    3 * STEPS + 60, a weight's gradient rows * STEPS; terms as large as 8 times the largest sum, as in the smaller model's test."""
+    set_mode(monkeypatch, mode)
+    torch.manual_seed(11)
+    size = 128
+    encoders = [mm.SequenceEncoder(size, V, 64, (32, 32), states=8, rank=3), mm.MLPEncoder(size, 6, (32, 32)),
+                mm.SequenceEncoder(size, V + 5, 24, (32, 32), states=4, rank=2), mm.MLPEncoder(size, 6, (32, 32))]
+    model = mm.MultiModN(size, encoders, [mm.LogisticDecoder(size) for _ in range(3)], 0.7, 0.4, device=torch.device("cuda"))
+    wide = copy.deepcopy(model).cpu().double()
+    data, y = batch(3, rows)
+    data, y = data + [data[1].flip(0)], torch.cat([y, y[:, :1].flip(0)], 1)
+    hist = mm.MultiModNHistory(["a", "b", "c"])
+    model.train_epoch([(data, y)], torch.optim.SGD(model.parameters(), 0.0), torch.nn.CrossEntropyLoss(), hist)
+    loss, grid = plain_step(wide, data, y)
+    bound = (2100 + 3 * STEPS + 60 + rows * STEPS) * 2.0 ** -24 * 8
+    assert rel_err(hist.loss["train"][0], grid.detach().numpy()) < 1e-5
+    for (n, p), g in zip(model.named_parameters(), torch.autograd.grad(loss, list(wide.parameters()))):
+        assert rel_err(p.grad.cpu().numpy(), g.numpy()) < bound, n
