@@ -128,6 +128,15 @@ Tensor state_pair(const Opt& state, const Opt& out_state) {
     NEED(a == b || a + n <= b || b + n <= a, "out_state overlaps state without being the same memory");
     return out;
 }
+// ... which no other operand shares: the kernels write it while other threads still read theirs
+void apart(const Tensor& out, const char* name, const Tensor& t) {
+    if (t.numel() == 0 || out.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const char *a = (const char*)out.data_ptr(), *b = (const char*)t.data_ptr();
+    NEED(a + out.nbytes() <= b || b + (last + 1) * t.element_size() <= a, std::string(name) + " shares memory with the state that the step writes");
+}
+void apart(const Tensor& out, const char* name, const Opt& t) { if (t) apart(out, name, *t); }
 void moved(const Tensor& t) {                                        // written through its address: autograd's saved copies are stale
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -266,6 +275,7 @@ Tensor conv_step(const Tensor& x, const Tensor& weight, const Opt& bias, bool si
     serving(x, weight, bias, state);
     const Tensor out = state_pair(state, out_state);
     Conv k(x, weight, bias, silu, {}, state, 2);
+    apart(out, "x", k.x); apart(out, "weight", k.weight); apart(out, "bias", k.bias);
     const On on(k.x);
     k.check(on);
     const Tensor y = at::empty(x.sizes(), k.x.options());
@@ -378,6 +388,8 @@ Tensor scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, const Tenso
     serving(x, dt, a, b, c, d, z, dt_bias, state);
     const Tensor out = state_pair(state, out_state);
     Scan k(x, dt, a, b, c, d, z, dt_bias, softplus, {}, state, 2);
+    apart(out, "x", k.x); apart(out, "dt", k.dt); apart(out, "a", k.a); apart(out, "b", k.b); apart(out, "c", k.c); apart(out, "d", k.d);
+    apart(out, "z", k.z); apart(out, "dt_bias", k.dt_bias);
     const On on(k.x);
     k.check(on);
     const Tensor y = at::empty(x.sizes(), k.x.options());

@@ -174,3 +174,19 @@ def test_captures_of_a_front_refuse_what_another_stream_holds():
             front(ids)
     torch.cuda.synchronize()
     assert torch.equal(features, front(ids))
+
+
+def test_one_step_forms_refuse_operands_inside_the_state():
+    """The step writes the state while other threads read their operands: x, b or a parameter that lies in it would be read before or after."""
+    z = torch.zeros
+    conv, scan = z(2, 3, 6), z(2, 6, 3)
+    w, a, x, b = z(6, 4), z(6, 3), z(2, 6), z(2, 3)
+    for call in (lambda: seq.causal_conv_step(conv[:, 2], w, state=conv), lambda: seq.causal_conv_step(x, conv.view(-1)[:24].view(6, 4), state=conv),
+                 lambda: seq.causal_conv_step(x, w, conv[0, 0], state=z(2, 3, 6), out_state=conv),
+                 lambda: seq.selective_scan_step(scan.view(2, 18)[:, :6], x, a, b, b, state=scan), lambda: seq.selective_scan_step(x, x, a, scan[:, 0], b, state=scan),
+                 lambda: seq.selective_scan_step(x, x, scan[0], b, b, state=scan), lambda: seq.selective_scan_step(x, x, a, b, b, state=z(2, 6, 3), out_state=scan, z=scan.view(2, 18)[:, 12:])):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    both = z(36 + 12)                                                         # side by side in one buffer is no overlap: only the CPU is refused
+    with pytest.raises(hip.MmnError):
+        seq.causal_conv_step(both[36:].view(2, 6), w, state=both[:36].view(2, 3, 6))
