@@ -7,7 +7,7 @@ import torch
 import multimodn_amd as mm
 from helpers import rel_err
 from test_hip_parity import KERNEL_MODES, set_mode
-from test_sequence_encoder import ROWS, STEPS, V, batch, build, plain_step
+from test_sequence_encoder import ROWS, S, STEPS, V, WIDTH, batch, build, plain_features, plain_step
 
 gpu = pytest.mark.gpu
 
@@ -132,3 +132,74 @@ def test_fronts_train_through_every_tier_of_the_chain(mode, rows, monkeypatch):
     assert rel_err(hist.loss["train"][0], grid.detach().numpy()) < 1e-5
     for (n, p), g in zip(model.named_parameters(), torch.autograd.grad(loss, list(wide.parameters()))):
         assert rel_err(p.grad.cpu().numpy(), g.numpy()) < bound, n
+
+
+@gpu
+@pytest.mark.parametrize("split", ["0", "1"])
+def test_fronts_beside_encoders_of_another_family(split, monkeypatch):
+    """A MIMIC_MLPEncoder (without dropout) and MLPDecoders take the chain through the generic tier's kernels: the front's gradients against 64
+    bits.  Bound as in the test of the tiers, with this model's sums (24 + 20, 16, 12 and their backward passes: under 300 for three encoders)."""
+    monkeypatch.setenv("MMN_GEN_SPLIT", split)
+    torch.manual_seed(12)
+    size, rows = 20, 33
+    encoders = [mm.SequenceEncoder(size, V, WIDTH, (16,), states=8, rank=3), mm.MIMIC_MLPEncoder(size, 6, (12,), 0.0),
+                mm.SequenceEncoder(size, V + 5, 8, (5, 7), torch.sigmoid, states=4, rank=2)]
+    model = mm.MultiModN(size, encoders, [mm.MLPDecoder(size, (9,)), mm.LogisticDecoder(size)], 0.7, 0.4, device=torch.device("cuda"))
+    wide = copy.deepcopy(model).cpu().double()
+    data, y = batch(3, rows)
+    model.train_epoch([(data, y)], torch.optim.SGD(model.parameters(), 0.0), torch.nn.CrossEntropyLoss())
+    state = wide.init_state.state_value.expand(rows, -1)
+    errors, change = [torch.stack([torch.nn.functional.cross_entropy(d(state), y[:, i]) for i, d in enumerate(wide.decoders)])], 0.0
+    for enc, x in zip(wide.encoders, data):
+        old = state
+        state = mm.MLPEncoder.forward(enc, state, plain_features(enc.front, x)) if isinstance(enc, mm.SequenceEncoder) else enc(state, x.double())
+        change = change + ((state - old) ** 2).mean()
+        errors.append(torch.stack([torch.nn.functional.cross_entropy(d(state), y[:, i]) for i, d in enumerate(wide.decoders)]))
+    loss = torch.stack(errors).mean() * wide.err_penalty + change / 3 * wide.state_change_penalty
+    bound = (300 + 3 * STEPS + 60 + rows * STEPS) * 2.0 ** -24 * 8
+    for (n, p), g in zip(model.named_parameters(), torch.autograd.grad(loss, list(wide.parameters()))):
+        assert rel_err(p.grad.cpu().numpy(), g.numpy()) < bound, n
+
+
+@gpu
+def test_fronts_of_no_rows_and_no_steps():
+    front = build(seed=4).encoders[0].front
+    assert not front(torch.zeros(3, 0, dtype=torch.int64, device="cuda")).any() and front(torch.zeros(0, 5, dtype=torch.int64, device="cuda")).shape == (0, WIDTH)
+    assert not front(torch.full((2, 4), -1, device="cuda")).any()
+    for ids in (torch.zeros(3, 0, dtype=torch.int64, device="cuda"), torch.full((2, 4), -1, device="cuda")):
+        front(ids).sum().backward()
+        assert all(p.grad is None or not p.grad.any() for p in front.parameters())
+
+
+@gpu
+def test_missing_ids_in_test_and_predict():
+    """test() skips the encoder of a batch with a missing id, as it does another modality's; predict() has no skip: its rows are NaN."""
+    model = build(seed=4)
+    plain = mm.MultiModN(S, [mm.MLPEncoder(S, e.n_features, e.hidden_layers, e.activation) for e in model.encoders],
+                         [mm.LogisticDecoder(S), mm.LogisticDecoder(S)], 0.7, 0.4, device=torch.device("cuda"))
+    plain.load_state_dict({k: v for k, v in model.state_dict().items() if ".front." not in k})
+    data, y = batch(5)
+    data[0] = data[0].float()
+    data[0][3, 2] = float("nan")
+    with torch.no_grad():
+        feats = [e.front(x.cuda()) if isinstance(e, mm.SequenceEncoder) else x.cuda() for e, x in zip(model.encoders, data)]
+    assert torch.isnan(feats[0][3]).all() and torch.isfinite(feats[0][[0, 1, 2]]).all()
+    crit = torch.nn.CrossEntropyLoss()
+    for r, s in zip(model.test([(data, y)], crit), plain.test([(feats, y.cuda())], crit)):
+        for a, b in zip(r, s):
+            assert torch.allclose(torch.as_tensor(a), torch.as_tensor(b), rtol=0, atol=0, equal_nan=True)
+    assert torch.equal(torch.isnan(torch.as_tensor(model.predict(data))), torch.isnan(torch.as_tensor(plain.predict(feats))))
+
+
+@gpu
+def test_autocast():
+    """Mixed precision around a front: the projections and what they feed in 16 bits, states and sums in 32."""
+    front = build(seed=4).encoders[0].front
+    ids = batch(5)[0][0].cuda()
+    want = front(ids)
+    with torch.autocast("cuda", torch.bfloat16):
+        got = front(ids)
+        got.sum().backward()
+    # x, z, u, dt, b, c and y are rounded to bf16 (2^-8 each, half of that on average): some ten such roundings of values up to 8 times the result
+    assert got.dtype == torch.float32 and rel_err(got.detach().cpu(), want.detach().cpu()) < 10 * 2.0 ** -8 * 8
+    assert all(torch.isfinite(p.grad).all() and p.grad.dtype == torch.float32 for p in front.parameters())
