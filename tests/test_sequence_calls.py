@@ -190,3 +190,31 @@ def test_one_step_forms_refuse_operands_inside_the_state():
     both = z(36 + 12)                                                         # side by side in one buffer is no overlap: only the CPU is refused
     with pytest.raises(hip.MmnError):
         seq.causal_conv_step(both[36:].view(2, 6), w, state=both[:36].view(2, 3, 6))
+
+
+@gpu
+@pytest.mark.parametrize("rows,steps", [(4, 30), (1, 2000), (1000, 20)])
+def test_states_of_one_step(rows, steps):
+    """a = -inf: nothing of a state is left at the next step, h = dt' x b.  Rows of every length, in segments and whole, and one step on."""
+    g = rng(46)
+    D, N = 10, 5
+    x, dt, b, c, h0 = normal(g, rows, steps, D), normal(g, rows, steps, D), normal(g, rows, steps, N), normal(g, rows, steps, N), normal(g, rows, D, N)
+    lengths = torch.randint(0, steps + 1, (rows,), generator=g)
+    lengths[0] = steps // 2 + 1
+    a = torch.full((D, N), -float("inf"), device="cuda")
+    y, state = seq.selective_scan(x, dt, a, b, c, lengths=lengths.cuda(), state=h0, return_state=True)
+    there = torch.arange(steps) < lengths[:, None]
+    wide = [t.cpu().double() for t in (x, dt, b, c)]
+    step = torch.nn.functional.softplus(wide[1])
+    h = (step * wide[0])[..., None] * wide[2][:, :, None]
+    want = torch.where(there[..., None], (h * wide[3][:, :, None]).sum(-1), 0.0)
+    mag = ((step + torch.sigmoid(wide[1]) * wide[1].abs()) * wide[0].abs())[..., None] * (wide[2] * wide[3]).abs()[:, :, None]
+    O.check(y, want, mag.sum(-1), N + 12, "y")
+    ends = (lengths - 1).clamp(min=0)
+    last = torch.where((lengths > 0)[:, None, None], h[torch.arange(rows), ends], h0.cpu().double())
+    last_mag = ((step + torch.sigmoid(wide[1]) * wide[1].abs()) * wide[0].abs())[..., None] * wide[2].abs()[:, :, None]
+    O.check(state, last, last_mag[torch.arange(rows), ends], 12, "state")
+    for t in (0, 1):
+        out = seq.selective_scan_step(x[:, t], dt[:, t], a, b[:, t], c[:, t], state=state)
+        O.check(state, h[:, t], last_mag[:, t], 12, "state of a step")
+        O.check(out, (h * wide[3][:, :, None]).sum(-1)[:, t], mag.sum(-1)[:, t], N + 12, "y of a step")
