@@ -218,3 +218,25 @@ def test_states_of_one_step(rows, steps):
         out = seq.selective_scan_step(x[:, t], dt[:, t], a, b[:, t], c[:, t], state=state)
         O.check(state, h[:, t], last_mag[:, t], 12, "state of a step")
         O.check(out, (h * wide[3][:, :, None]).sum(-1)[:, t], mag.sum(-1)[:, t], N + 12, "y of a step")
+
+
+@gpu
+@pytest.mark.parametrize("rows,steps,growth", [(1000, 300, 1.0), (9000, 200, 1.0), (3, 300, 1.0), (3, 300, 200.0), (1000, 40, 200.0)])
+def test_growing_states_of_few_channels(rows, steps, growth):
+    """Six channels of a wave's 64 lanes, a > 0 and steps so small that nothing grows much: the lanes without a channel, whose step would be
+    softplus(0), add nothing to the gradients of b and c.  All rows are alike."""
+    g = rng(47)
+    D, N = 6, 3
+    x, dy = torch.randn(1, steps, D, generator=g), torch.randn(1, steps, D, generator=g)
+    dt = torch.full((1, steps, D), -10.0)
+    b, c = torch.randn(1, steps, N, generator=g), torch.randn(1, steps, N, generator=g)
+    a, h0, ds = torch.full((D, N), growth), torch.randn(1, D, N, generator=g), torch.randn(1, D, N, generator=g)
+    want = O.scan(x, dt, a, b.unsqueeze(2), c.unsqueeze(2), None, None, None, True, None, h0, dy, ds)
+    case = [t.expand(rows, *t.shape[1:]).contiguous().cuda() for t in (x, dt, b, c, h0, dy, ds)]
+    y, state, saved = seq.selective_scan_forward(case[0], case[1], a.cuda(), case[2], case[3], state=case[4], return_state=True)
+    grads = seq.selective_scan_grad(case[5], saved, case[6])
+    n = 3 * steps + 12 + N + 24
+    for i in (0, rows - 1):
+        O.check(y[i:i + 1], *want["y"], n, "y")
+        for name in ("x", "dt", "b", "c", "state"):
+            O.check(getattr(grads, name)[i:i + 1], *want["dstate" if name == "state" else name], 2 * n + D, "d" + name)
